@@ -61,6 +61,13 @@ extern "C" {
                             queries needing several passes, and other shapes, by the fp32 table
                             lookups */
 
+/* normalisation of tokens written into pages (tms_page_write) */
+#define TMS_NORM_NONE 0 /* y = h */
+#define TMS_NORM_L2 1   /* y = h / max(|h|, eps) */
+#define TMS_NORM_RMS 2  /* y = h / sqrt(mean(h^2) + eps) * weight */
+
+#define TMS_PAGED_MAX_D 256 /* widest token of a paged corpus */
+
 /* dense output modes */
 #define TMS_OUT_SCORE 0     /* out[q * n_docs + doc] = sum_i max_j <Q_qi, D_j>                 */
 #define TMS_OUT_TOKEN_MAX 1 /* out[(q * n_docs + doc) * nq + i] = max_j <Q_qi, D_j> (V1 output) */
@@ -244,6 +251,73 @@ TMS_API int tms_topk_pack(const float* vals, const int64_t* ids, int64_t rows, i
                           int64_t* packed, void* stream);
 TMS_API int tms_topk_merge_packed(const int64_t* gathered, int64_t world, int64_t rows, int64_t k,
                                   float* out_vals, int64_t* out_ids, void* stream);
+
+/* ---------------------------------------------------------------- paged 8-bit corpora */
+/* No reference function (its corpora are fixed tensors). Python: tilemaxsim_b200.PagedCorpus and
+ * page_tables / select_page_tables / page_write / page_read / paged_maxsim.
+ *
+ * A pool holds n_pages pages of page_size (16, 32, 64 or 128) token rows: codes (n_pages, page_size,
+ * d) e4m3, 16-byte aligned, and scales (n_pages) fp32; a token's value is scale * code. A document
+ * owns ceil(length / page_size) pages: entries [page_offsets[i], page_offsets[i + 1]) of page_ids,
+ * in order. page_docs names each entry's document. Rows behind a document's last token repeat that
+ * token. d is a multiple of 16, at most TMS_PAGED_MAX_D. Whatever the tables hold, no call reads or
+ * writes outside its arrays: an entry whose page id lies outside the pool is skipped. */
+
+TMS_API size_t tms_page_tables_workspace_size(int64_t n_docs);
+
+/* The page tables and token slots of n_docs documents, from their lengths. Document i's length is
+ * lengths[i], or lengths[doc_ids[i]] when doc_ids != NULL (an id outside [0, n_lengths) and a
+ * negative length count as 0 tokens; the same id may come twice). Its pages are taken from `pages`
+ * (n_src_pages): in order over all documents when src_offsets == NULL (a free list), else from
+ * entry src_offsets[doc_ids ? doc_ids[i] : i] on (a store's own tables: documents are selected).
+ * Writes page_offsets and token_offsets (n_docs + 1, running counts); every entry of page_ids and
+ * page_docs (page_capacity): -1 past the last page, and page id -1 where `pages` has none; and,
+ * unless slots == NULL, every entry of slots (token_capacity): page id * page_size + row of each
+ * token, -1 where it has no page or table entry and past the last token. What the capacities do not
+ * hold is left out (compare them with page_offsets[n_docs] and token_offsets[n_docs]). A capacity of
+ * (token_capacity + n_docs * (page_size - 1)) / page_size pages always holds token_capacity tokens.
+ * page_capacity, n_docs < 2^31. */
+TMS_API int tms_page_tables(const int64_t* lengths, int64_t n_lengths, const int64_t* doc_ids,
+                            int64_t n_docs, const int64_t* src_offsets, const int32_t* pages,
+                            int64_t n_src_pages, int64_t page_size, int64_t* page_offsets,
+                            int64_t* token_offsets, int32_t* page_ids, int32_t* page_docs,
+                            int64_t page_capacity, int64_t* slots, int64_t token_capacity,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* Writes the documents of the tables (as tms_page_tables makes them) into their pages: token h =
+ * x (+ residual), normalised as `norm` says (fp64 sums), scale = max |y| / 448 over the page's
+ * tokens rounded to fp32, code = e4m3(y / scale) rounded once to nearest. x, residual: dtype, rows of d
+ * elements stride_token apart; padded != 0: document i starts at i * stride_doc and has n_rows
+ * rows at most; else its tokens are rows token_offsets[i].. of n_rows. Tokens past n_rows read as
+ * zeros. weight: (d) dtype, only with TMS_NORM_RMS, NULL for ones. A page with a NaN or an infinity
+ * among its normalised values gets scale NaN and codes NaN. Buffers 16-byte aligned, strides
+ * multiples of 16 bytes. Pages that the tables do not name are left as they were; a page named
+ * twice ends up with either content, or a mixture. */
+TMS_API int tms_page_write(const void* x, int dtype, int64_t n_rows, int64_t stride_doc,
+                           int64_t stride_token, int padded, const void* residual,
+                           const void* weight, int norm, float eps, int64_t d, int64_t page_size,
+                           const int64_t* page_offsets, const int64_t* token_offsets,
+                           const int32_t* page_ids, const int32_t* page_docs, int64_t n_docs,
+                           int64_t page_capacity, void* codes, float* scales, int64_t n_pages,
+                           void* stream);
+
+/* out (n_slots, d) out_dtype: scale * code of each slot (fp32 product, rounded to out_dtype); a
+ * slot outside the pool gives zeros. */
+TMS_API int tms_page_read(const void* codes, const float* scales, int64_t n_pages,
+                          int64_t page_size, int64_t d, const int64_t* slots, int64_t n_slots,
+                          void* out, int out_dtype, void* stream);
+
+TMS_API size_t tms_paged_workspace_size(int64_t n_queries, int64_t nq, int64_t n_docs);
+
+/* out[q * n_docs + i] = sum_t max over the values v of document i's pages of <Q[q,t,:], v> (fp32
+ * accumulation); a document without pages scores -inf, one with a NaN page NaN. Q: (n_queries, nq,
+ * d) fp16 or bf16, 16-byte aligned. n_pages * page_size < 2^31. */
+TMS_API int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, int64_t nq, int64_t d,
+                             const void* codes, const float* scales, int64_t n_pages,
+                             int64_t page_size, const int64_t* page_offsets,
+                             const int32_t* page_ids, const int32_t* page_docs, int64_t n_docs,
+                             int64_t page_capacity, float* out, void* workspace,
+                             size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- introspection and test hooks */
 

@@ -1,0 +1,526 @@
+"""The paged 8-bit corpus operators on the GPU against their plain restatement in 64 bits."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as R
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def _rng(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _np(t):
+    return t.cpu().numpy()
+
+
+def _same_tables(got, want):
+    for name, g, w in zip(("page_offsets", "page_ids", "page_docs", "token_offsets", "slots"), got, want):
+        np.testing.assert_array_equal(_np(g), w, err_msg=name)
+
+
+# ------------------------------------------------------------------------------------------ tables
+
+@pytest.mark.parametrize("lengths,page", [
+    ([1], 16), ([0], 32), ([0, 0, 5, 0], 16), ([31, 32, 33, 0, 1, 64, 65], 32), ([700, 1, 128, 127, 129, 0], 128),
+    ([1] * 70 + [0] * 40 + [65] * 3, 64)])
+def test_tables_small(lengths, page, cuda_device):
+    from tilemaxsim_b200 import page_tables
+    total = sum(lengths)
+    need = sum(-(-n // page) for n in lengths)
+    pages = torch.randperm(need + 3, generator=_rng(need)).to(torch.int32)
+    for bound in (total, total + 77):
+        t = page_tables(torch.tensor(lengths).to(cuda_device), page, pages.to(cuda_device), bound)
+        _same_tables(t, R.tables(lengths, page, pages.tolist(), bound))
+    t = page_tables(torch.tensor(lengths, dtype=torch.int32).to(cuda_device), page, pages.to(cuda_device), total, slots=False)
+    assert t.slots is None
+    # a free list that runs out: the entries it has no page for are -1
+    short = pages[:need // 2]
+    t = page_tables(torch.tensor(lengths).to(cuda_device), page, short.to(cuda_device), total)
+    _same_tables(t, R.tables(lengths, page, short.tolist(), total))
+
+
+@pytest.mark.parametrize("n,page,hi", [(1023, 32, 300), (1024, 16, 40), (1025, 64, 5), (4097, 32, 70), (20011, 16, 33)])
+def test_tables_many_documents(n, page, hi, cuda_device):
+    from tilemaxsim_b200 import page_tables, select_page_tables
+    g = _rng(n)
+    lengths = torch.randint(0, hi, (n,), generator=g)
+    lengths[n // 3: n // 3 + 50] = 0
+    total, need = int(lengths.sum()), int(((lengths + page - 1) // page).sum())
+    pages = torch.randperm(need, generator=g).to(torch.int32)
+    t = page_tables(lengths.to(cuda_device), page, pages.to(cuda_device), total)
+    want = R.tables(lengths, page, pages.tolist(), total)
+    _same_tables(t, want)
+    ids = torch.randint(-3, n + 3, (1500,), generator=g)
+    bound = 1500 * hi
+    s = select_page_tables(lengths.to(cuda_device), page, t.page_offsets, t.page_ids, ids.to(cuda_device), bound)
+    _same_tables(s, R.tables(lengths, page, want[1].tolist(), bound, ids, want[0]))
+
+
+def test_tables_nothing(cuda_device):
+    from tilemaxsim_b200 import page_tables, select_page_tables
+    none = torch.zeros(0, dtype=torch.int64, device=cuda_device)
+    pages = torch.arange(3, dtype=torch.int32, device=cuda_device)
+    t = page_tables(none, 32, pages, 5)
+    _same_tables(t, R.tables([], 32, [0, 1, 2], 5))
+    t = select_page_tables(none, 32, torch.zeros(1, dtype=torch.int64, device=cuda_device), pages[:0],
+                           torch.tensor([0, 4], device=cuda_device), 0)
+    assert _np(t.page_offsets).tolist() == [0, 0, 0]
+
+
+def test_tables_one_long_document_and_negative_lengths(cuda_device):
+    from tilemaxsim_b200 import page_tables
+    lengths = [5, -7, 100001, 3]
+    pages = list(range(4000))[::-1]
+    t = page_tables(torch.tensor(lengths).to(cuda_device), 32, torch.tensor(pages, dtype=torch.int32).to(cuda_device), 100009)
+    _same_tables(t, R.tables(lengths, 32, pages, 100009))
+
+
+def test_tables_bound_too_small(cuda_device):
+    """A bound below the token count cuts the outputs off; nothing is written past them."""
+    from tilemaxsim_b200 import page_tables
+    lengths = [40, 50, 60]
+    t = page_tables(torch.tensor(lengths).to(cuda_device), 16, torch.arange(20, dtype=torch.int32).to(cuda_device), 30)
+    want = R.tables(lengths, 16, list(range(20)), 30)
+    _same_tables(t, want)
+
+
+# ------------------------------------------------------------------------------------------ write and read
+
+def _layout(lengths, page, seed, spare=2):
+    from tilemaxsim_b200 import page_tables
+    need = sum(-(-n // page) for n in lengths)
+    pages = torch.randperm(need + spare, generator=_rng(seed)).to(torch.int32).cuda()
+    return page_tables(torch.tensor(lengths).cuda(), page, pages, sum(lengths)), need + spare
+
+
+def _check_written(codes, scales, tables, lengths, tokens, page):
+    """tokens: float64 normalised tokens of all documents, in order."""
+    c, s = codes.cpu().double().numpy(), scales.cpu().double().numpy()
+    ids, po = _np(tables.page_ids), _np(tables.page_offsets)
+    at = 0
+    for i, n in enumerate(lengths):
+        for k in range(-(-n // page)):
+            rows = tokens[at + k * page: at + min(n, (k + 1) * page)]
+            pid = ids[po[i] + k]
+            scale = np.abs(rows).max() / R.E4M3_MAX
+            # one rounding to fp32 (to nothing below half its least value)
+            assert abs(s[pid] - scale) <= max(scale * 2.0 ** -24 * 1.0001, 2.0 ** -150), (i, k)
+            if s[pid] == 0:
+                assert not c[pid].any()
+                continue
+            t = np.clip(rows / s[pid], -R.E4M3_MAX, R.E4M3_MAX)
+            off = np.abs(c[pid][:len(rows)] - t)
+            assert (off <= R.half_step(t) * (1 + 1e-9)).all(), (i, k, off.max())
+            assert (c[pid][len(rows):] == c[pid][len(rows) - 1]).all(), (i, k)
+        at += n
+    return c, s
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("norm,residual,weight", [("l2", False, False), ("l2", True, False), ("rms", True, True),
+                                                   ("rms", False, False), ("none", False, False), ("none", True, False)])
+@pytest.mark.parametrize("page,d,lengths", [
+    (16, 16, [1, 15, 16, 17, 0, 40]), (32, 128, [1, 0, 31, 32, 33, 100]), (64, 96, [64, 130, 5]), (128, 256, [1, 200, 128]),
+    (32, 48, [7, 33])])
+def test_write(page, d, lengths, norm, residual, weight, dtype, cuda_device):
+    from tilemaxsim_b200 import page_read, page_write
+    g = _rng(page + d)
+    x = torch.randn(sum(lengths), d, generator=g).to(dtype)
+    x[0] = 0  # a row of zeros has no direction
+    r = torch.randn(sum(lengths), d, generator=g).to(dtype) if residual else None
+    w = (1 + 0.2 * torch.randn(d, generator=g)).to(dtype) if weight else None
+    t, n_pages = _layout(lengths, page, 5)
+    codes = torch.full((n_pages, page, d), 1.5, device=cuda_device).to(torch.float8_e4m3fn)
+    scales = torch.full((n_pages,), 7.0, device=cuda_device)
+    out = page_write(x.cuda(), t, codes, scales, residual=r.cuda() if residual else None,
+                     weight=w.cuda() if weight else None, norm=norm)
+    assert out[0] is codes and out[1] is scales
+    f = lambda v: None if v is None else v.double().numpy()  # noqa: E731
+    c, s = _check_written(codes, scales, t, lengths, R.normalise(f(x), f(r), f(w), norm), page)
+    free = sorted(set(range(n_pages)) - set(_np(t.page_ids)[:_np(t.page_offsets)[-1]].tolist()))
+    assert len(free) == 2 and (s[free] == 7.0).all() and (c[free] == 1.5).all()  # left as they were
+    # read back: the fp32 product rounded once to each type
+    slots = _np(t.slots)
+    want = c.reshape(-1, d)[slots] * s[slots // page][:, None]
+    for dt in DTYPES:
+        got = page_read(codes, scales, t.slots, dt).cpu().double().numpy()
+        step = torch.finfo(dt).eps / 2 + 2.0 ** -24
+        assert (np.abs(got - want) <= np.abs(want) * step + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_write_padded_batch_and_strides(dtype, cuda_device):
+    """A padded batch with garbage (NaN) behind each document, and views with other strides, write the
+    same pages as the ragged tokens."""
+    from tilemaxsim_b200 import page_write
+    lengths, L, d, page = [9, 0, 33, 50, 1], 50, 64, 32
+    g = _rng(3)
+    x = torch.randn(5, L, d, generator=g).to(dtype).cuda()
+    r = torch.randn(5, L, d, generator=g).to(dtype).cuda()
+    keep = torch.arange(L)[None] < torch.tensor(lengths)[:, None]
+    xp, rp = x.clone(), r.clone()
+    xp[~keep], rp[~keep] = float("nan"), float("inf")
+    t, n_pages = _layout(lengths, page, 1)
+
+    def write(x, r):
+        codes = torch.zeros(n_pages, page, d, device=cuda_device).to(torch.float8_e4m3fn)
+        scales = torch.zeros(n_pages, device=cuda_device)
+        page_write(x, t, codes, scales, residual=r)
+        return _np(codes.view(torch.uint8)), _np(scales)
+
+    want = write(x[keep.cuda()], r[keep.cuda()])
+    big = torch.full((5, L + 3, 2 * d + 16), float("nan"), dtype=dtype, device=cuda_device)
+    big[:, 1:L + 1, 16:d + 16] = xp
+    odd = torch.full((5, L, d + 1), float("nan"), dtype=dtype, device=cuda_device)
+    odd[:, :, 1:] = xp
+    for xv, rv in ((xp, rp), (big[:, 1:L + 1, 16:d + 16], rp), (odd[:, :, 1:], rp),
+                   (xp.transpose(0, 1).contiguous().transpose(0, 1), rp)):
+        got = write(xv, rv)
+        np.testing.assert_array_equal(got[0], want[0])
+        np.testing.assert_array_equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("norm", ["l2", "rms", "none"])
+def test_write_non_finite_poisons_its_page_only(value, norm, cuda_device):
+    from tilemaxsim_b200 import page_read, page_write, paged_maxsim
+    lengths, d, page = [20, 40, 10], 32, 16
+    x = torch.randn(70, d, generator=_rng(8)).half()
+    x[20 + 17, 3] = value  # document 1, page 1
+    t, n_pages = _layout(lengths, page, 2, spare=0)
+    codes = torch.zeros(n_pages, page, d, device=cuda_device).to(torch.float8_e4m3fn)
+    scales = torch.zeros(n_pages, device=cuda_device)
+    page_write(x.cuda(), t, codes, scales, norm=norm)
+    got = page_read(codes, scales, t.slots, torch.float32)
+    bad = torch.zeros(70, dtype=torch.bool)
+    bad[36:52] = True
+    assert torch.isnan(got.cpu()).all(1).tolist() == bad.tolist()
+    s = _np(paged_maxsim(torch.randn(2, 5, d, generator=_rng(9)).half().cuda(), codes, scales, t))
+    assert np.isnan(s[:, 1]).all() and np.isfinite(s[:, [0, 2]]).all()
+
+
+def test_write_extreme_magnitudes(cuda_device):
+    """Values near the ends of fp32, and pages whose scale rounds to nothing."""
+    from tilemaxsim_b200 import page_write
+    d, page, lengths = 16, 16, [4, 4, 4, 4]
+    x = torch.randn(16, d, generator=_rng(1))
+    x[:4] *= 1e38 / x[:4].abs().max()
+    x[4:8] *= 1e-30
+    x[8:12] *= 1e-43 / x[8:12].abs().max()
+    x[12:] = 1e-45
+    t, n_pages = _layout(lengths, page, 2)
+    codes = torch.zeros(n_pages, page, d, device=cuda_device).to(torch.float8_e4m3fn)
+    scales = torch.zeros(n_pages, device=cuda_device)
+    page_write(x.cuda(), t, codes, scales, norm="none")
+    _check_written(codes, scales, t, lengths, x.double().numpy(), page)
+
+
+def test_write_malformed_tables_stay_inside(cuda_device):
+    """Entries that name no page of the pool, no document, or rows that x does not have."""
+    from tilemaxsim_b200 import PageTables, page_write
+    d, page = 32, 16
+    i64 = lambda *v: torch.tensor(v, dtype=torch.int64, device=cuda_device)  # noqa: E731
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda_device)  # noqa: E731
+    codes = torch.ones(4, page, d, device=cuda_device).to(torch.float8_e4m3fn)
+    scales = torch.ones(4, device=cuda_device)
+    x = torch.randn(20, d, generator=_rng(4)).half().cuda()
+    t = PageTables(i64(0, 2, 4, 6), i32(-1, 9, 1, 2, 3, 2147483647), i32(0, 0, 7, -1, 2, 2), i64(0, 20, 60, 90), None)
+    page_write(x, t, codes, scales)  # entry 4: document 2 starts at row 60 of 20
+    t = t._replace(token_offsets=i64(-5, 10, 1 << 40, -(1 << 50)))
+    page_write(x, t, codes, scales)
+    t = t._replace(page_offsets=i64(-(1 << 60), 1 << 60, 3, 6), page_docs=i32(0, 0, 1, 1, 2, 2))
+    page_write(x, t, codes, scales)
+    assert (scales[:3] == 1).all()
+
+
+def test_read_slots_outside_the_pool(cuda_device):
+    from tilemaxsim_b200 import page_read
+    codes = torch.randn(3, 16, 48, generator=_rng(1)).cuda().to(torch.float8_e4m3fn)
+    scales = torch.tensor([1.0, 2.0, 0.5], device=cuda_device)
+    slots = torch.tensor([0, -1, 47, 48, 1 << 40, -(1 << 50), 16], device=cuda_device)
+    got = page_read(codes, scales, slots, torch.float32).cpu()
+    flat = codes.float().cpu().view(48, 48) * scales.cpu().repeat_interleave(16)[:, None]
+    want = torch.zeros(7, 48)
+    want[0], want[2], want[6] = flat[0], flat[47], flat[16]
+    assert torch.equal(got, want)
+    assert page_read(codes, scales, slots[:0]).shape == (0, 48)
+
+
+# ------------------------------------------------------------------------------------------ scores
+
+def _corpus(lengths, page, d, seed, dtype=torch.bfloat16):
+    """A written pool and each document's stored tokens in float64."""
+    from tilemaxsim_b200 import page_write
+    x = torch.randn(sum(lengths), d, generator=_rng(seed)).to(dtype).cuda()
+    t, n_pages = _layout(lengths, page, seed)
+    codes = torch.full((n_pages, page, d), float("nan"), device="cuda").to(torch.float8_e4m3fn)
+    scales = torch.full((n_pages,), float("nan"), device="cuda")
+    page_write(x, t, codes, scales)
+    slots = t.slots.cpu()
+    flat = codes.float().cpu().view(-1, d)[slots].double() * scales.cpu().double()[slots // page][:, None]
+    return t, codes, scales, [v.numpy() for v in flat.split(lengths)]
+
+
+def _queries(bq, nq, d, seed, dtype):
+    return torch.nn.functional.normalize(torch.randn(bq, nq, d, generator=_rng(seed)), dim=-1).to(dtype).cuda()
+
+
+def _check_scores(got, Q, docs):
+    q = Q.cpu().double().numpy()
+    want, bound = R.scores(q, docs), R.score_bound(q, docs)
+    got = _np(got).astype(np.float64)
+    empty = np.isinf(want)
+    np.testing.assert_array_equal(got[empty], want[empty])
+    off = np.abs(np.where(empty, 0, got) - np.where(empty, 0, want))
+    assert (off <= bound).all(), (off - bound).max()
+
+
+RAGGED = [1, 0, 15, 16, 17, 31, 32, 33, 63, 64, 65, 0, 0, 127, 128, 129, 300, 2, 1, 1, 0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("bq,nq,d", [(1, 1, 128), (1, 32, 128), (2, 32, 64), (3, 20, 96), (1, 33, 128), (5, 32, 16),
+                                      (1, 128, 128), (2, 77, 256), (17, 32, 128)])
+def test_scores(bq, nq, d, page, dtype, cuda_device):
+    from tilemaxsim_b200 import paged_maxsim
+    t, codes, scales, docs = _corpus(RAGGED, page, d, bq * 100 + d)
+    Q = _queries(bq, nq, d, 7, dtype)
+    got = paged_maxsim(Q, codes, scales, t)
+    assert got.shape == (bq, len(RAGGED)) and got.dtype == torch.float32
+    _check_scores(got, Q, docs)
+    assert torch.equal(got, paged_maxsim(Q, codes, scales, t))
+    if bq == 1:
+        assert torch.equal(got[0], paged_maxsim(Q[0], codes, scales, t))
+
+
+@pytest.mark.parametrize("bq,nq,d,page,n,hi,dtype", [
+    (1, 32, 128, 32, 3001, 300, torch.bfloat16), (1, 32, 128, 16, 2003, 40, torch.float16),
+    (2, 32, 128, 32, 1501, 300, torch.float16), (4, 32, 64, 64, 1500, 200, torch.bfloat16),
+    (64, 32, 128, 32, 700, 200, torch.bfloat16), (33, 40, 128, 16, 400, 100, torch.float16),
+    (20, 8, 256, 128, 300, 300, torch.float16), (1, 32, 128, 32, 9000, 2, torch.bfloat16)])
+def test_scores_larger(bq, nq, d, page, n, hi, dtype, cuda_device):
+    from tilemaxsim_b200 import paged_maxsim
+    lengths = torch.randint(0, hi + 1, (n,), generator=_rng(n)).tolist()
+    t, codes, scales, docs = _corpus(lengths, page, d, n)
+    Q = _queries(bq, nq, d, 3, dtype)
+    _check_scores(paged_maxsim(Q, codes, scales, t), Q, docs)
+
+
+def test_scores_long_documents(cuda_device):
+    from tilemaxsim_b200 import paged_maxsim
+    lengths = [20000, 1, 7001, 0, 30000]
+    t, codes, scales, docs = _corpus(lengths, 32, 128, 1)
+    Q = _queries(3, 32, 128, 3, torch.bfloat16)
+    _check_scores(paged_maxsim(Q, codes, scales, t), Q, docs)
+
+
+@pytest.mark.parametrize("lengths", [[0], [0, 0, 0], [1], [3]])
+def test_scores_hardly_anything(lengths, cuda_device):
+    from tilemaxsim_b200 import paged_maxsim
+    t, codes, scales, docs = _corpus(lengths, 32, 128, 1)
+    Q = _queries(2, 40, 128, 3, torch.float16)
+    _check_scores(paged_maxsim(Q, codes, scales, t), Q, docs)
+    assert paged_maxsim(Q[:0], codes, scales, t).shape == (0, len(lengths))
+
+
+def test_scores_query_values(cuda_device):
+    """Zero rows, rows far apart in magnitude, outliers and subnormal values in one query; fp32 queries
+    are rounded to fp16."""
+    from tilemaxsim_b200 import paged_maxsim
+    t, codes, scales, docs = _corpus(RAGGED, 32, 128, 4)
+    for dtype, tiny, big in ((torch.float16, 6e-8, 6e4), (torch.bfloat16, 1e-38, 1e30)):
+        Q = _queries(1, 40, 128, 5, torch.float32)
+        Q[0, 1] = 0
+        Q[0, 2] *= big / 2
+        Q[0, 3] *= tiny * 20
+        Q[0, 4, 7] = 100.0
+        Q[0, 5] = 0
+        Q[0, 5, 9] = 1.0
+        Q = Q.to(dtype)
+        for i in range(40):  # one row at a time: the bound is each row's own
+            _check_scores(paged_maxsim(Q[:, i:i + 1], codes, scales, t), Q[:, i:i + 1], docs)
+        _check_scores(paged_maxsim(Q, codes, scales, t), Q, docs)
+    Q = _queries(2, 32, 128, 5, torch.float32)
+    assert torch.equal(paged_maxsim(Q, codes, scales, t), paged_maxsim(Q.half(), codes, scales, t))
+
+
+def test_scores_skip_entries_outside_the_pool(cuda_device):
+    """A page id outside the pool is left out; a document all of whose pages are is empty."""
+    from tilemaxsim_b200 import paged_maxsim
+    t, codes, scales, docs = _corpus([40, 20, 33, 64], 32, 64, 4)
+    ids = t.page_ids.clone()
+    ids[1], ids[2], ids[3] = -1, 1 << 30, codes.shape[0]  # document 0's second page, 1's only one, 2's first
+    Q = _queries(3, 32, 64, 5, torch.bfloat16)
+    got = paged_maxsim(Q, codes, scales, t._replace(page_ids=ids))
+    _check_scores(got, Q, [docs[0][:32], docs[1][:0], docs[2][32:], docs[3]])
+
+
+def test_scores_malformed_offsets_stay_inside(cuda_device):
+    from tilemaxsim_b200 import paged_maxsim
+    t, codes, scales, _ = _corpus([40, 20, 33, 64], 32, 64, 4)
+    Q = _queries(3, 32, 64, 5, torch.bfloat16)
+    good = paged_maxsim(Q, codes, scales, t)
+    for off in ([-5, 9, 2, 1 << 40, 3], [7, 7, 7, 7, 7], [1 << 62] * 5, [0, 0, 0, 0, -1], [6, 5, 4, 3, 2]):
+        bad = t._replace(page_offsets=torch.tensor(off, dtype=torch.int64, device=cuda_device))
+        assert paged_maxsim(Q, codes, scales, bad).shape == (3, 4)
+    docs = t.page_docs.clone()
+    docs[:] = torch.tensor([5, -1, 1 << 30, 0, 3, 2, 1, 0][:docs.numel()], dtype=torch.int32)
+    assert paged_maxsim(Q, codes, scales, t._replace(page_docs=docs)).shape == (3, 4)
+    assert torch.equal(paged_maxsim(Q, codes, scales, t), good)
+
+
+def test_scores_other_stream_and_graph(cuda_device):
+    from tilemaxsim_b200 import GraphedStep, paged_maxsim
+    t, codes, scales, docs = _corpus(RAGGED, 32, 128, 4)
+    Q = _queries(2, 40, 128, 5, torch.bfloat16)
+    want = paged_maxsim(Q, codes, scales, t)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = paged_maxsim(Q, codes, scales, t)
+    side.synchronize()
+    assert torch.equal(got, want)
+    a = GraphedStep(lambda q: paged_maxsim(q, codes, scales, t), Q)
+    b = GraphedStep(lambda q: paged_maxsim(q, codes, scales, t), Q)
+    Q2 = _queries(2, 40, 128, 6, torch.bfloat16)
+    assert torch.equal(a(Q), want.cpu())
+    assert torch.equal(b(Q2), paged_maxsim(Q2, codes, scales, t).cpu())
+    assert torch.equal(a(Q), want.cpu())
+
+
+# ------------------------------------------------------------------------------------------ the corpus
+
+def test_corpus_life(cuda_device):
+    """Documents are added (ragged, padded), scored, selected, read, removed and added again."""
+    from tilemaxsim_b200 import PagedCorpus, maxsim_batched
+    d, page = 64, 16
+    c = PagedCorpus(d, n_pages=60, max_docs=40, page_size=page)
+    kept: dict[int, torch.Tensor] = {}
+
+    def add(lengths, padded, seed):
+        n = len(lengths)
+        x = torch.randn(n, max(max(lengths), 1), d, generator=_rng(seed)).half().cuda()
+        rows = [x[i, :m] for i, m in enumerate(lengths)]
+        ids = c.add(x if padded else torch.cat(rows), torch.tensor(lengths) if padded else lengths)
+        for i, r in zip(ids.tolist(), rows):
+            kept[i] = torch.nn.functional.normalize(r.float(), dim=-1).cpu()
+        return ids.tolist()
+
+    Q = _queries(3, 32, d, 5, torch.float16)
+
+    def check():
+        n = c.n_docs
+        tok, off = c.tokens(list(range(n)), torch.float32)
+        tok, off = tok.cpu(), off.tolist()
+        docs = [tok[off[i]:off[i + 1]] for i in range(n)]
+        for i in range(n):
+            assert docs[i].shape == kept[i].shape
+            if len(docs[i]):  # e4m3 with a scale of the page's largest value: half a step of 2^-3, or of 2^-9 / 448 of it
+                most = kept[i].abs().max()
+                assert ((docs[i] - kept[i]).abs() <= kept[i].abs() * 2.0 ** -4 * 1.001 + most * 2.0 ** -10 / 448 * 1.001).all()
+        _check_scores(c.score_queries(Q), Q, [v.double().numpy() for v in docs])
+        pick = torch.tensor([n - 1, 0, n // 2, 0, n + 5, -1])
+        sel = c.score_queries(Q, pick.cuda())
+        assert torch.equal(sel[:, :4], c.score_queries(Q)[:, pick[:4].cuda()]) and torch.isinf(sel[:, 4:]).all()
+        v, i = c.search(Q, 5)
+        vs, is_ = c.search(Q, 3, pick[:3].cuda())
+        assert torch.equal(v[:, 0], c.score_queries(Q).amax(1)) and set(is_.flatten().tolist()) <= set(pick[:3].tolist())
+        # the same tokens through the dense kernel: fp16 rounding of the tokens, its 1e-3 tolerance
+        t16, o16 = c.tokens(list(range(n)))
+        dense = maxsim_batched(Q, t16, o16)
+        fin = torch.isfinite(dense)
+        assert torch.equal(torch.isfinite(c.score_queries(Q)), fin)
+        torch.testing.assert_close(c.score_queries(Q)[fin], dense[fin], rtol=1e-3, atol=1e-3)
+
+    assert add([5, 16, 17, 0, 40], False, 1) == [0, 1, 2, 3, 4]
+    check()
+    add([33, 1, 100], True, 2)
+    check()
+    free = c.n_free
+    c.remove(torch.tensor([2, 7, 2, 3]))
+    c.remove([2])
+    for i in (2, 7):
+        kept[i] = kept[i][:0]
+    assert c.n_free == free + 2 + 7
+    check()
+    assert add([100, 90, 17], False, 3) == [8, 9, 10]
+    check()
+    before = [t.clone() for t in c.tables[:4]]
+    with pytest.raises(ValueError, match="pages are needed"):
+        c.add(torch.zeros(1000, d).half().cuda(), [1000])
+    with pytest.raises(ValueError, match="no room"):
+        c.add(torch.zeros(0, d).half().cuda(), [0] * 30)
+    with pytest.raises(ValueError, match="sum"):
+        c.add(torch.zeros(5, d).half().cuda(), [4])
+    with pytest.raises(ValueError, match="fit"):
+        c.add(torch.zeros(1, 5, d).half().cuda(), [6])
+    with pytest.raises(ValueError, match="negative"):
+        c.add(torch.zeros(5, d).half().cuda(), [6, -1])
+    with pytest.raises(TypeError):
+        c.add(torch.zeros(5, d).double().cuda(), [5])
+    with pytest.raises(IndexError):
+        c.remove([11])
+    assert c.n_docs == 11 and all(torch.equal(a, b) for a, b in zip(before, c.tables[:4]))
+    c.remove(list(range(11)))
+    assert c.n_free == 60 and sorted(c._free.tolist()) == list(range(60))
+    assert torch.isinf(c.score_queries(Q)).all()
+    for i in list(kept):
+        kept[i] = kept[i][:0]
+    add([60 * 16], False, 9)
+    assert c.n_free == 0
+    check()
+
+
+def test_corpus_captured_search_sees_removals(cuda_device):
+    from tilemaxsim_b200 import GraphedStep, PagedCorpus
+    c = PagedCorpus(128, n_pages=100, max_docs=50)
+    g = _rng(2)
+    c.add(torch.randn(600, 128, generator=g).half().cuda(), [100, 200, 50, 250])
+    Q = _queries(2, 32, 128, 5, torch.float16)
+    step = GraphedStep(lambda q: c.search(q, 2), Q)
+    v, i = step(Q)
+    want_v, want_i = c.search(Q, 2)
+    assert torch.equal(v, want_v.cpu()) and torch.equal(i, want_i.cpu())
+    c.remove([int(want_i[0, 0])])
+    c.add(torch.randn(64, 128, generator=g).half().cuda(), [64])
+    v, i = step(Q)
+    want = c.score_queries(Q)[:, :4].topk(2)
+    assert torch.equal(v, want.values.cpu()) and torch.equal(i, want.indices.cpu())
+
+
+def test_ivf_candidates_reranked_in_place(cuda_device):
+    """IVFIndex takes a PagedCorpus as the tokens it reranks: the scores are the corpus's own."""
+    from tilemaxsim_b200 import IVFIndex, PagedCorpus
+    g = _rng(6)
+    lengths = torch.randint(1, 60, (200,), generator=g)
+    off = torch.zeros(201, dtype=torch.int64)
+    off[1:] = torch.cumsum(lengths, 0)
+    x = torch.nn.functional.normalize(torch.randn(int(off[-1]), 64, generator=g), dim=-1).half().cuda()
+    cent = torch.nn.functional.normalize(torch.randn(50, 64, generator=g), dim=-1).half().cuda()
+    index = IVFIndex(cent, (x @ cent.T).argmax(1), off.cuda())
+    corpus = PagedCorpus(64, n_pages=700, max_docs=200, page_size=16)
+    corpus.add(x, lengths)
+    Q = _queries(4, 32, 64, 5, torch.float16)
+    vals, ids = index.search(Q, corpus, 7, nprobe=2)
+    bitmaps, cand = index.candidates(Q, 2)
+    full = corpus.score_queries(Q)
+    for q in range(4):
+        mine = [d for d in cand.tolist() if int(bitmaps[q, d >> 5]) >> (d & 31) & 1]
+        best = sorted(mine, key=lambda d: (-float(full[q, d]), d))[:7]
+        assert ids[q, :len(best)].tolist() == best
+        assert torch.equal(vals[q, :len(best)], full[q, best])
+    gone = [int(ids[0, 0]), int(ids[1, 0])]
+    corpus.remove(gone)
+    vals2, ids2 = index.search(Q, corpus, 7, nprobe=2)
+    assert not set(gone) & set(ids2.flatten().tolist()) and torch.equal(vals2[0, :6], vals[0, 1:])
+    assert PagedCorpus(64, 4, 4).n_docs == 0
+    with pytest.raises(ValueError, match="documents"):
+        index.search(Q, PagedCorpus(64, 4, 4), 7, nprobe=2)

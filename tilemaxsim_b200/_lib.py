@@ -25,6 +25,8 @@ TMS_ERR_BAD_OFFSETS = 7
 
 TMS_F16, TMS_BF16, TMS_F32 = 0, 1, 2
 TMS_OUT_SCORE, TMS_OUT_TOKEN_MAX = 0, 1
+TMS_NORM_NONE, TMS_NORM_L2, TMS_NORM_RMS = 0, 1, 2
+TMS_PAGED_MAX_D = 256
 TMS_PQ_FAST, TMS_PQ_EXACT, TMS_PQ_PRECISE = 0, 1, 2
 
 DTYPE_CODE = {torch.float16: TMS_F16, torch.bfloat16: TMS_BF16, torch.float32: TMS_F32}
@@ -60,6 +62,15 @@ SIGNATURES = {
     "tms_residual_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
     "tms_residual_maxsim": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i64, _vp, _i64,
                                    _i64, _vp, _vp, _sz, _vp]),
+    "tms_page_tables_workspace_size": (_sz, [_i64]),
+    "tms_page_tables": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64,
+                               _vp, _sz, _vp]),
+    "tms_page_write": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _i32, ctypes.c_float, _i64, _i64, _vp,
+                              _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "tms_page_read": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _vp]),
+    "tms_paged_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "tms_paged_maxsim": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp,
+                                _vp, _sz, _vp]),
     "tms_topk_workspace_size": (_sz, [_i64, _i64, _i64]),
     "tms_topk": (_i32, [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
 }

@@ -13,6 +13,8 @@ ColBERTv2 / PLAID index stores (the ``codes`` of ``ResidualMaxSim``):
 3. the union's documents are gathered into one contiguous ragged corpus (``tms_gather_docs``) and
    scored for the whole query batch by ONE dense MaxSim launch; a query's scores of documents that
    only other queries probed are masked (``tms_mask_candidates``), and each query keeps its top-k.
+   Given a ``PagedCorpus`` instead of a token matrix, the candidates are scored where they lie:
+   their page tables are selected, no token is copied.
 
 A document's MaxSim score does not depend on the rest of the corpus, so the scores equal those of
 scoring the full corpus, bit for bit; the search returns the exact top-k of each query's own
@@ -26,6 +28,7 @@ import torch
 
 from . import _lib
 from .maxsim import maxsim_batched, topk
+from .paged import PagedCorpus
 
 
 class IVFIndex:
@@ -89,13 +92,17 @@ class IVFIndex:
             n_cand = int(count.item())  # sizes the gathered corpus: one host synchronisation
         return bitmaps, cand[:n_cand]
 
-    def search(self, Qb: torch.Tensor, D_tokens: torch.Tensor, k: int, nprobe: int
+    def search(self, Qb: torch.Tensor, D_tokens: torch.Tensor | PagedCorpus, k: int, nprobe: int
                ) -> tuple[torch.Tensor, torch.Tensor]:
         """Top-k of each query among its own candidates, by exact MaxSim over D_tokens (the corpus
-        the index was built for). Returns (scores (B_q, k) fp32, doc ids (B_q, k) int64); a query
-        with fewer than k candidates is padded with (-inf, -1)."""
+        the index was built for: its token matrix, or a PagedCorpus whose document ids are the
+        index's; documents removed from it are not returned). Returns (scores (B_q, k) fp32, doc ids
+        (B_q, k) int64); a query with fewer than k candidates is padded with (-inf, -1)."""
         lib = _lib.load()
-        _lib.require_cuda(Qb, D_tokens)
+        paged = isinstance(D_tokens, PagedCorpus)
+        _lib.require_cuda(Qb, D_tokens.codes if paged else D_tokens)
+        if paged and D_tokens.n_docs < self.n_docs:
+            raise ValueError(f"the corpus has {D_tokens.n_docs} documents, the index {self.n_docs}")
         Bq = Qb.shape[0]
         bitmaps, cand = self.candidates(Qb, nprobe)
         n_cand = cand.numel()
@@ -103,6 +110,27 @@ class IVFIndex:
         ids = torch.full((Bq, k), -1, dtype=torch.int64, device=self.device)
         if n_cand == 0 or Bq == 0:
             return vals, ids
+        with torch.cuda.device(self.device):
+            scores = D_tokens.score_queries(Qb, cand) if paged else self._score_gathered(Qb, D_tokens, cand)
+            rc = lib.tms_mask_candidates(ctypes.c_void_p(scores.data_ptr()), Bq, n_cand, n_cand,
+                                         ctypes.c_void_p(cand.data_ptr()),
+                                         ctypes.c_void_p(bitmaps.data_ptr()), self.n_docs,
+                                         ctypes.c_float(float("nan")),
+                                         ctypes.c_void_p(_lib.stream_handle(self.device)))
+            _lib.check(rc, "tms_mask_candidates")
+        kk = min(k, n_cand)
+        v, col = topk(scores, kk)  # columns ascend with document id: the tie rule carries over
+        pad = torch.isnan(v)  # ranks after every candidate: not a candidate of this query
+        if paged:
+            pad |= v == float("-inf")  # removed from the corpus since the index was built
+        vals[:, :kk] = v.masked_fill(pad, float("-inf"))
+        ids[:, :kk] = cand[col].masked_fill(pad, -1)
+        return vals, ids
+
+    def _score_gathered(self, Qb: torch.Tensor, D_tokens: torch.Tensor, cand: torch.Tensor) -> torch.Tensor:
+        """(B_q, n_cand) scores of the candidates, gathered into one ragged corpus."""
+        lib = _lib.load()
+        n_cand = cand.numel()
         D_tokens = D_tokens.contiguous()
         row_bytes = D_tokens.shape[1] * D_tokens.element_size()
         with torch.cuda.device(self.device):
@@ -120,15 +148,4 @@ class IVFIndex:
                                      ctypes.c_void_p(g_off.data_ptr()), total,
                                      ctypes.c_void_p(G.data_ptr()), stream)
             _lib.check(rc, "tms_gather_docs")
-            scores = maxsim_batched(Qb, G[:total], g_off)
-            rc = lib.tms_mask_candidates(ctypes.c_void_p(scores.data_ptr()), Bq, n_cand, n_cand,
-                                         ctypes.c_void_p(cand.data_ptr()),
-                                         ctypes.c_void_p(bitmaps.data_ptr()), self.n_docs,
-                                         ctypes.c_float(float("nan")), stream)
-            _lib.check(rc, "tms_mask_candidates")
-        kk = min(k, n_cand)
-        v, col = topk(scores, kk)  # columns ascend with document id: the tie rule carries over
-        pad = torch.isnan(v)  # ranks after every candidate: not a candidate of this query
-        vals[:, :kk] = v.masked_fill(pad, float("-inf"))
-        ids[:, :kk] = cand[col].masked_fill(pad, -1)
-        return vals, ids
+        return maxsim_batched(Qb, G[:total], g_off)

@@ -1,0 +1,403 @@
+"""An 8-bit corpus in pages: documents can join and leave it, and are scored where they lie.
+
+A pool of pages holds the tokens: each page has ``page_size`` rows of d e4m3 values and one fp32
+scale, so a token costs one byte a dimension. A document owns as many pages as its length needs,
+anywhere in the pool; its page table lists them. Four operators work on that layout, each one a
+stream-ordered call of the C ABI:
+
+    page_tables / select_page_tables   lengths -> page tables and the slot of every token
+    page_write                         tokens (+ residual) -> normalised, e4m3 with a scale a page
+    paged_maxsim                       queries x documents -> MaxSim scores
+    page_read                          slots -> tokens
+
+``PagedCorpus`` keeps a pool, its free pages and the tables of its documents, and builds on them.
+The reference has no such corpus: its corpora are fixed tensors (src/flash_maxsim_kernel.py:248-273).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .maxsim import topk
+
+PAGE_SIZES = (16, 32, 64, 128)
+_NORMS = {"none": _lib.TMS_NORM_NONE, "l2": _lib.TMS_NORM_L2, "rms": _lib.TMS_NORM_RMS}
+_EPS = {"none": 0.0, "l2": 1e-12, "rms": 1e-6}
+
+
+class PageTables(NamedTuple):
+    """Where n documents live. page_offsets (n + 1,) int64: document i owns table entries
+    [page_offsets[i], page_offsets[i + 1]); page_ids, page_docs (capacity,) int32: each entry's page
+    and document, -1 past the last; token_offsets (n + 1,) int64: running token counts; slots
+    (tokens,) int64: page id * page_size + row of every token, -1 past the last (or None)."""
+    page_offsets: torch.Tensor
+    page_ids: torch.Tensor
+    page_docs: torch.Tensor
+    token_offsets: torch.Tensor
+    slots: torch.Tensor | None
+
+
+def _ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
+    return ctypes.c_void_p(t.data_ptr() if t is not None else 0)
+
+
+def _page_size(page_size: int) -> int:
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+    return int(page_size)
+
+
+def _ints(t: torch.Tensor, dtype: torch.dtype, name: str) -> torch.Tensor:
+    if t.dim() != 1 or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise ValueError(f"{name} must be a 1-D integer tensor, got {t.dtype} {tuple(t.shape)}")
+    return t.to(dtype).contiguous()
+
+
+def _tables_call(lengths, doc_ids, src_offsets, pages, page_size, n_tokens, with_slots) -> PageTables:
+    lib = _lib.load()
+    given = [t for t in (lengths, doc_ids, src_offsets, pages) if t is not None]
+    dev = _lib.require_cuda(*given)
+    n_docs = lengths.numel() if doc_ids is None else doc_ids.numel()
+    capacity = (n_tokens + n_docs * (page_size - 1)) // page_size
+    with torch.cuda.device(dev):
+        def empty(n, dtype):
+            return torch.empty(n, dtype=dtype, device=dev)
+        out = PageTables(empty(n_docs + 1, torch.int64), empty(capacity, torch.int32), empty(capacity, torch.int32),
+                         empty(n_docs + 1, torch.int64), empty(n_tokens, torch.int64) if with_slots else None)
+        ws_bytes = lib.tms_page_tables_workspace_size(n_docs)
+        ws, ws_ptr = _lib.workspace(ws_bytes, dev, align=256)
+        rc = lib.tms_page_tables(
+            _ptr(lengths), lengths.numel(), _ptr(doc_ids), n_docs, _ptr(src_offsets), _ptr(pages), pages.numel(),
+            page_size, _ptr(out.page_offsets), _ptr(out.token_offsets), _ptr(out.page_ids), _ptr(out.page_docs),
+            capacity, _ptr(out.slots), n_tokens, ctypes.c_void_p(ws_ptr), ws_bytes,
+            ctypes.c_void_p(_lib.stream_handle(dev)))
+        _lib.check(rc, "tms_page_tables")
+        del ws
+    return out
+
+
+def page_tables(lengths: torch.Tensor, page_size: int, free_pages: torch.Tensor, n_tokens: int,
+                slots: bool = True) -> PageTables:
+    """The tables of new documents of the given lengths (n,), whose pages are the first ones of
+    ``free_pages`` (1-D page ids), in order. n_tokens: the sum of the lengths, or a bound on it (it
+    sizes the outputs, without a host synchronisation). Where the free list runs out, page ids and
+    slots are -1: compare page_offsets[-1] with free_pages.numel() to see it."""
+    page_size = _page_size(page_size)
+    if n_tokens < 0:
+        raise ValueError(f"n_tokens must not be negative, got {n_tokens}")
+    lengths = _ints(lengths, torch.int64, "lengths")
+    free_pages = _ints(free_pages, torch.int32, "free_pages")
+    return _tables_call(lengths, None, None, free_pages, page_size, int(n_tokens), slots)
+
+
+def select_page_tables(lengths: torch.Tensor, page_size: int, page_offsets: torch.Tensor, page_ids: torch.Tensor,
+                       doc_ids: torch.Tensor, n_tokens: int, slots: bool = True) -> PageTables:
+    """The tables of documents ``doc_ids`` (n,) of a store with the given lengths (N,), page_offsets
+    (N + 1,) and page_ids: candidates are scored or read where they lie. The same id may come more
+    than once; an id outside the store is an empty document. n_tokens bounds their tokens."""
+    page_size = _page_size(page_size)
+    if n_tokens < 0:
+        raise ValueError(f"n_tokens must not be negative, got {n_tokens}")
+    lengths = _ints(lengths, torch.int64, "lengths")
+    page_offsets = _ints(page_offsets, torch.int64, "page_offsets")
+    if page_offsets.numel() < lengths.numel():
+        raise ValueError(f"{lengths.numel()} lengths need as many page_offsets, got {page_offsets.numel()}")
+    return _tables_call(lengths, _ints(doc_ids, torch.int64, "doc_ids"), page_offsets,
+                        _ints(page_ids, torch.int32, "page_ids"), page_size, int(n_tokens), slots)
+
+
+def _check_pool(codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, int]:
+    if codes.dim() != 3 or codes.dtype != torch.float8_e4m3fn or not codes.is_contiguous():
+        raise ValueError("codes must be a contiguous (n_pages, page_size, d) float8_e4m3fn tensor, got "
+                         f"{codes.dtype} {tuple(codes.shape)}")
+    n_pages, page_size, d = codes.shape
+    _page_size(page_size)
+    if d % 16 or not 0 < d <= _lib.TMS_PAGED_MAX_D:
+        raise ValueError(f"d must be a multiple of 16, at most {_lib.TMS_PAGED_MAX_D}, got {d}")
+    if scales.shape != (n_pages,) or scales.dtype != torch.float32 or not scales.is_contiguous():
+        raise ValueError(f"scales must be a contiguous ({n_pages},) float32 tensor, got {scales.dtype} "
+                         f"{tuple(scales.shape)}")
+    if codes.data_ptr() % 16:
+        raise ValueError("codes must be 16-byte aligned")
+    return n_pages, page_size, d
+
+
+def _check_tables(t: PageTables) -> int:
+    if any(x.dim() != 1 or x.dtype != torch.int64 or not x.is_contiguous() for x in (t.page_offsets, t.token_offsets)):
+        raise ValueError("page_offsets and token_offsets must be contiguous 1-D int64 tensors")
+    if any(x.dim() != 1 or x.dtype != torch.int32 or not x.is_contiguous() for x in (t.page_ids, t.page_docs)):
+        raise ValueError("page_ids and page_docs must be contiguous 1-D int32 tensors")
+    if t.page_ids.numel() != t.page_docs.numel():
+        raise ValueError("page_ids and page_docs must have the same length")
+    n = t.page_offsets.numel() - 1
+    if n < 0 or t.token_offsets.numel() != n + 1:
+        raise ValueError("page_offsets and token_offsets must have n_docs + 1 entries each")
+    return n
+
+
+def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales: torch.Tensor, *,
+               residual: torch.Tensor | None = None, weight: torch.Tensor | None = None, norm: str = "l2",
+               eps: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Writes documents into their pages: h = x + residual; y = h / max(|h|, eps) for norm "l2", h /
+    sqrt(mean(h^2) + eps) * weight for "rms", h for "none"; each page's scale is its largest |y|
+    over 448, its codes are e4m3(y / scale).
+
+    x: the tokens of all documents (T, d), document i's at token_offsets[i].., or a padded batch
+    (n_docs, L, d) whose document i has its tokens in the first rows (lengths must not exceed L);
+    fp16, bf16 or fp32; residual: same shape and dtype. codes and scales are updated in place and
+    returned; pages that the tables do not name keep their content."""
+    lib = _lib.load()
+    if norm not in _NORMS:
+        raise ValueError(f"norm must be one of {sorted(_NORMS)}, got {norm!r}")
+    if weight is not None and norm != "rms":
+        raise ValueError("weight goes with norm='rms' only")
+    eps = _EPS[norm] if eps is None else float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    n_pages, page_size, d = _check_pool(codes, scales)
+    n_docs = _check_tables(tables)
+    dev = _lib.require_cuda(x, codes, scales, tables.page_offsets, tables.page_ids, tables.page_docs,
+                            tables.token_offsets, *(t for t in (residual, weight) if t is not None))
+    if x.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {x.dtype}; use float16, bfloat16 or float32")
+    if x.dim() not in (2, 3) or x.shape[-1] != d:
+        raise ValueError(f"expected x (T, {d}) or (n_docs, L, {d}), got {tuple(x.shape)}")
+    padded = x.dim() == 3
+    if padded and x.shape[0] != n_docs:
+        raise ValueError(f"a padded x has a document for each of the tables' {n_docs}, got {x.shape[0]}")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("residual must have the shape and dtype of x")
+    if weight is not None and weight.shape != (d,):
+        raise ValueError(f"weight must be ({d},), got {tuple(weight.shape)}")
+    rows = 16 // x.element_size()  # elements of 16 bytes
+
+    def fits(t):
+        return t.stride(-1) == 1 and all(s % rows == 0 and s >= 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
+
+    with torch.cuda.device(dev):
+        if not fits(x) or (residual is not None and (not fits(residual) or residual.stride() != x.stride())):
+            x = x.clone(memory_format=torch.contiguous_format)
+            residual = None if residual is None else residual.clone(memory_format=torch.contiguous_format)
+        if weight is not None:
+            weight = weight.to(x.dtype).contiguous()
+            weight = weight if weight.data_ptr() % 16 == 0 else weight.clone()
+        rc = lib.tms_page_write(
+            _ptr(x), _lib.DTYPE_CODE[x.dtype], x.shape[-2], x.stride(0) if padded else 0, x.stride(-2), int(padded),
+            _ptr(residual), _ptr(weight), _NORMS[norm], eps, d, page_size, _ptr(tables.page_offsets),
+            _ptr(tables.token_offsets), _ptr(tables.page_ids), _ptr(tables.page_docs), n_docs,
+            tables.page_ids.numel(), _ptr(codes), _ptr(scales), n_pages, ctypes.c_void_p(_lib.stream_handle(dev)))
+        _lib.check(rc, "tms_page_write")
+    return codes, scales
+
+
+def page_read(codes: torch.Tensor, scales: torch.Tensor, slots: torch.Tensor,
+              dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """The tokens in the given slots (n,) as (n, d) fp16, bf16 or fp32 values scale * code; a slot
+    outside the pool (-1 among them) gives a row of zeros."""
+    lib = _lib.load()
+    n_pages, page_size, d = _check_pool(codes, scales)
+    if dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {dtype}; use float16, bfloat16 or float32")
+    slots = _ints(slots, torch.int64, "slots")
+    dev = _lib.require_cuda(codes, scales, slots)
+    with torch.cuda.device(dev):
+        out = torch.empty((slots.numel(), d), dtype=dtype, device=dev)
+        rc = lib.tms_page_read(_ptr(codes), _ptr(scales), n_pages, page_size, d, _ptr(slots), slots.numel(),
+                               _ptr(out), _lib.DTYPE_CODE[dtype], ctypes.c_void_p(_lib.stream_handle(dev)))
+        _lib.check(rc, "tms_page_read")
+    return out
+
+
+def paged_maxsim(Qb: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tables: PageTables) -> torch.Tensor:
+    """MaxSim of every query against every document of the tables, straight from the pages.
+
+    Qb: (B_q, Nq, d) or (Nq, d), fp16 or bf16 (fp32 is rounded to fp16). Returns fp32 (B_q, n_docs),
+    or (n_docs,) for a single 2-D query. A document without pages scores -inf, one with a NaN among
+    its pages NaN."""
+    lib = _lib.load()
+    n_pages, page_size, d = _check_pool(codes, scales)
+    n_docs = _check_tables(tables)
+    single = Qb.dim() == 2
+    if single:
+        Qb = Qb.unsqueeze(0)
+    dev = _lib.require_cuda(Qb, codes, scales, tables.page_offsets, tables.page_ids, tables.page_docs)
+    if Qb.dim() != 3 or Qb.shape[2] != d:
+        raise ValueError(f"expected Q (B_q, Nq, {d}) or (Nq, {d}), got {tuple(Qb.shape)}")
+    if Qb.dtype == torch.float32:
+        Qb = Qb.to(torch.float16)
+    if Qb.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"unsupported dtype {Qb.dtype}; use float16, bfloat16 or float32")
+    Bq, Nq, _ = Qb.shape
+    if Nq == 0:
+        raise ValueError("a query needs at least one token")
+    with torch.cuda.device(dev):
+        Qb = Qb.contiguous()
+        Qb = Qb if Qb.data_ptr() % 16 == 0 else Qb.clone()
+        out = torch.empty((Bq, n_docs), dtype=torch.float32, device=dev)
+        if Bq > 0 and n_docs > 0:
+            ws_bytes = lib.tms_paged_workspace_size(Bq, Nq, n_docs)
+            ws, ws_ptr = _lib.workspace(ws_bytes, dev, align=256)
+            rc = lib.tms_paged_maxsim(
+                _ptr(Qb), _lib.DTYPE_CODE[Qb.dtype], Bq, Nq, d, _ptr(codes), _ptr(scales), n_pages, page_size,
+                _ptr(tables.page_offsets), _ptr(tables.page_ids), _ptr(tables.page_docs), n_docs,
+                tables.page_ids.numel(), _ptr(out), ctypes.c_void_p(ws_ptr), ws_bytes,
+                ctypes.c_void_p(_lib.stream_handle(dev)))
+            _lib.check(rc, "tms_paged_maxsim")
+            del ws
+    return out[0] if single else out
+
+
+class PagedCorpus:
+    """A pool of pages with room for n_pages * page_size tokens and max_docs documents.
+
+    Documents get ascending ids in the order they are added; a removed document's id is not given
+    out again and scores -inf. All device buffers are allocated here and updated in place, so a
+    captured search (``GraphedStep``) sees later additions to the documents it was captured for
+    being removed, and never reads memory that was freed; documents added after the capture are not
+    in its output. ``add`` and ``remove`` synchronise with the host; order them against searches on
+    other streams as with any tensor that one stream writes and another reads."""
+
+    def __init__(self, d: int, n_pages: int, max_docs: int, page_size: int = 32,
+                 device: torch.device | str = "cuda"):
+        self.page_size = _page_size(page_size)
+        if d % 16 or not 0 < d <= _lib.TMS_PAGED_MAX_D:
+            raise ValueError(f"d must be a multiple of 16, at most {_lib.TMS_PAGED_MAX_D}, got {d}")
+        if n_pages < 1 or max_docs < 1 or n_pages * page_size >= 1 << 31 or max_docs >= 1 << 31:
+            raise ValueError("n_pages and max_docs must be positive, n_pages * page_size and max_docs below 2^31, got "
+                             f"{n_pages} pages of {page_size} and {max_docs}")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"tilemaxsim_b200 scores CUDA tensors only (no CPU fallback); got {device}")
+        self.d, self.n_pages, self.max_docs = d, n_pages, max_docs
+        self.codes = torch.zeros(n_pages, self.page_size, d, dtype=torch.float8_e4m3fn, device=device)
+        self.scales = torch.zeros(n_pages, dtype=torch.float32, device=device)
+        self.device = self.codes.device
+        self._lengths = torch.zeros(max_docs, dtype=torch.int64, device=device)
+        self._page_offsets = torch.zeros(max_docs + 1, dtype=torch.int64, device=device)
+        self._token_offsets = torch.zeros(max_docs + 1, dtype=torch.int64, device=device)
+        self._page_ids = torch.full((n_pages,), -1, dtype=torch.int32, device=device)
+        self._page_docs = torch.full((n_pages,), -1, dtype=torch.int32, device=device)
+        # free pages, the next ones to give out at the end
+        self._free = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=device)
+        self._host_lengths: list[int] = []
+        self.n_free = n_pages
+
+    @property
+    def n_docs(self) -> int:
+        """Documents added so far, removed ones included."""
+        return len(self._host_lengths)
+
+    @property
+    def tables(self) -> PageTables:
+        """The tables of all documents (views of the corpus's own buffers, without slots)."""
+        n = self.n_docs
+        return PageTables(self._page_offsets[:n + 1], self._page_ids, self._page_docs, self._token_offsets[:n + 1], None)
+
+    def _pages_of(self, lengths) -> int:
+        return sum((n + self.page_size - 1) // self.page_size for n in lengths)
+
+    def add(self, x: torch.Tensor, lengths: torch.Tensor | list[int], *, residual: torch.Tensor | None = None,
+            weight: torch.Tensor | None = None, norm: str = "l2", eps: float | None = None) -> torch.Tensor:
+        """Adds documents of the given lengths, their tokens in x as page_write takes them (ragged
+        (T, d) or padded (n, L, d)). Returns their ids (n,) int64. Raises ValueError, with the corpus
+        as it was, when the pool or the document table has no room."""
+        host = [int(n) for n in (lengths.tolist() if isinstance(lengths, torch.Tensor) else lengths)]
+        n, n_tok, first = len(host), sum(host), self.n_docs
+        if any(m < 0 for m in host):
+            raise ValueError("lengths must not be negative")
+        if x.dim() == 2 and x.shape[0] != n_tok:
+            raise ValueError(f"x has {x.shape[0]} tokens, the lengths sum to {n_tok}")
+        if x.dim() == 3 and (x.shape[0] != n or max(host, default=0) > x.shape[1]):
+            raise ValueError(f"lengths do not fit a padded batch of shape {tuple(x.shape)}")
+        need = self._pages_of(host)
+        if need > self.n_free:
+            raise ValueError(f"{need} pages are needed, {self.n_free} are free")
+        if first + n > self.max_docs:
+            raise ValueError(f"no room for {n} documents: {first} of {self.max_docs} are taken")
+        ids = torch.arange(first, first + n, device=self.device)
+        if n == 0:
+            return ids
+        with torch.cuda.device(self.device):
+            dev_lengths = torch.tensor(host, dtype=torch.int64, device=self.device)
+            free = self._free[self.n_free - need:self.n_free].flip(0)
+            t = page_tables(dev_lengths, self.page_size, free, n_tok, slots=False)
+            page_write(x, t, self.codes, self.scales, residual=residual, weight=weight, norm=norm, eps=eps)
+            used = self.n_pages - self.n_free
+            self._page_ids[used:used + need] = t.page_ids[:need]
+            self._page_docs[used:used + need] = t.page_docs[:need] + first
+            self._page_offsets[first + 1:first + 1 + n] = t.page_offsets[1:] + used
+            self._page_offsets[first + 1 + n:] = used + need
+            self._token_offsets[first + 1:first + 1 + n] = t.token_offsets[1:] + self._token_offsets[first]
+            self._token_offsets[first + 1 + n:] = self._token_offsets[first + n].clone()
+            self._lengths[first:first + n] = dev_lengths
+        self._host_lengths += host
+        self.n_free -= need
+        return ids
+
+    def _host_ids(self, doc_ids: torch.Tensor | list[int]) -> list[int]:
+        ids = [int(i) for i in (doc_ids.tolist() if isinstance(doc_ids, torch.Tensor) else doc_ids)]
+        if any(i < 0 or i >= self.n_docs for i in ids):
+            raise IndexError(f"document ids must be in [0, {self.n_docs})")
+        return ids
+
+    def remove(self, doc_ids: torch.Tensor | list[int]) -> None:
+        """Removes documents and frees their pages. An id may come twice; a document that is removed
+        already, or empty, is left as it is."""
+        ids = sorted({i for i in self._host_ids(doc_ids) if self._host_lengths[i] > 0})
+        if not ids:
+            return
+        freed = self._pages_of(self._host_lengths[i] for i in ids)
+        used = self.n_pages - self.n_free
+        with torch.cuda.device(self.device):
+            gone = torch.zeros(self.max_docs, dtype=torch.bool, device=self.device)
+            gone[torch.tensor(ids, device=self.device)] = True
+            out = gone[self._page_docs[:used].long()]
+            pages, docs = self._page_ids[:used].clone(), self._page_docs[:used].clone()
+            self._free[self.n_free:self.n_free + freed] = pages[out]
+            self._page_ids[:used - freed] = pages[~out]
+            self._page_docs[:used - freed] = docs[~out]
+            self._page_ids[used - freed:used] = -1
+            self._page_docs[used - freed:used] = -1
+            self._lengths[gone] = 0
+            shift = self.page_size - 1
+            self._page_offsets[1:] = torch.cumsum((self._lengths + shift) // self.page_size, 0)
+            self._token_offsets[1:] = torch.cumsum(self._lengths, 0)
+        for i in ids:
+            self._host_lengths[i] = 0
+        self.n_free += freed
+
+    def select(self, doc_ids: torch.Tensor, n_tokens: int | None = None, slots: bool = False) -> PageTables:
+        """The tables of the given documents (an id outside the corpus is an empty document).
+        n_tokens bounds their tokens; by default the longest document's length for each."""
+        doc_ids = _ints(doc_ids, torch.int64, "doc_ids")
+        if n_tokens is None:
+            n_tokens = doc_ids.numel() * max(self._host_lengths, default=0)
+        n = self.n_docs
+        return select_page_tables(self._lengths[:n], self.page_size, self._page_offsets[:n + 1], self._page_ids, doc_ids,
+                                  n_tokens, slots=slots)
+
+    def score_queries(self, Qb: torch.Tensor, doc_ids: torch.Tensor | None = None) -> torch.Tensor:
+        """Qb (B_q, Nq, d) or (Nq, d) -> fp32 scores (B_q, n) or (n,) of all documents, or of doc_ids
+        (n,) in their order."""
+        tables = self.tables if doc_ids is None else self.select(doc_ids)
+        return paged_maxsim(Qb, self.codes, self.scales, tables)
+
+    def search(self, Qb: torch.Tensor, k: int, doc_ids: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The k best documents of each query, of all or of the candidates doc_ids (n,): scores
+        (B_q, k) fp32 and ids (B_q, k) int64, by score descending and id ascending."""
+        scores = self.score_queries(Qb, doc_ids)
+        if doc_ids is None:
+            return topk(scores, k)
+        return topk(scores, k, ids=doc_ids.to(torch.int64).expand(scores.shape).contiguous())
+
+    def tokens(self, doc_ids: torch.Tensor | list[int], dtype: torch.dtype = torch.float16
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+        """The stored tokens of the given documents: (T, d) values and (n + 1,) int64 offsets, the
+        layout maxsim_batched and save_shard take."""
+        ids = self._host_ids(doc_ids)
+        n_tok = sum(self._host_lengths[i] for i in ids)
+        t = self.select(torch.tensor(ids, dtype=torch.int64, device=self.device), n_tok, slots=True)
+        return page_read(self.codes, self.scales, t.slots, dtype), t.token_offsets
