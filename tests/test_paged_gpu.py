@@ -322,6 +322,28 @@ def test_scores_long_documents(cuda_device):
     _check_scores(paged_maxsim(Q, codes, scales, t), Q, docs)
 
 
+@pytest.mark.parametrize("bq,page", [(1, 32), (2, 16), (4, 64), (20, 32)])
+def test_scores_long_streams(bq, page, cuda_device):
+    """Enough documents that every part of the corpus takes many steps, and parts end at different ones:
+    a query of a batch, and a document of a corpus, score what they score alone."""
+    from tilemaxsim_b200 import paged_maxsim
+    lengths = torch.randint(0, 201, (20000,), generator=_rng(1)).tolist()
+    t, codes, scales, docs = _corpus(lengths, page, 128, 3)
+    Q = _queries(bq, 32, 128, 3, torch.bfloat16)
+    got = paged_maxsim(Q, codes, scales, t)
+    pick = torch.randperm(20000, generator=_rng(2))[:400].tolist()
+    _check_scores(got[:, pick], Q, [docs[i] for i in pick])
+    best = torch.full((20000, bq * 32), float("-inf"), device=cuda_device)
+    used = t.page_ids >= 0
+    ids = t.page_ids[used].long()
+    for a in range(0, ids.numel(), 20000):  # float32 over the whole corpus: every document, coarsely
+        i = ids[a:a + 20000]
+        tok = codes.view(torch.uint8)[i].view(torch.float8_e4m3fn).float() * scales[i][:, None, None]
+        s = (tok.view(-1, 128) @ Q.float().view(-1, 128).T).view(i.numel(), page, -1).amax(1)
+        best.scatter_reduce_(0, t.page_docs[used][a:a + 20000].long()[:, None].expand_as(s), s, "amax")
+    torch.testing.assert_close(got, best.view(20000, bq, 32).sum(-1).T, rtol=1e-5, atol=1e-4)
+
+
 @pytest.mark.parametrize("lengths", [[0], [0, 0, 0], [1], [3]])
 def test_scores_hardly_anything(lengths, cuda_device):
     from tilemaxsim_b200 import paged_maxsim
