@@ -118,14 +118,35 @@ __device__ __forceinline__ float max_columns(const uint32_t* r) {
   return max3_nan(max3_nan(m[0], m[1], m[2]), max_nan(m[3], m[4]), rest);
 }
 
-// D(tmem) (+)= A * B^T, both K-major e4m3 in shared memory, fp32 accumulation.
-__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                       uint32_t accumulate) {
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(r));
+  return r;
+}
+// D(tmem) (+)= A * B^T, both K-major e4m3 in shared memory, fp32 accumulation, issued by the lane
+// whose `leader` is set. The whole warp runs the loop around it: the descriptors then stay in
+// uniform registers (an issue loop under "lane == 0" cost about 600 clocks a K chunk).
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar),
+      "r"(leader)
       : "memory");
 }
 
@@ -357,40 +378,44 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const PagedArgs 
     const uint32_t tmem = *tmem_slot;
     if (warp == 1) {
       // ---------------------------------------------------------------- MMA issue
-      if (lane == 0) {
-        constexpr uint32_t idesc = make_idesc(128, TN, 0);  // e4m3 operands, fp32 accumulator
-        int s = 0;
-        uint32_t ph = 0, u = 0;
-        bool ok = true;
-        for (int t = 0; ok && t < n_tiles; ++t) {
-          if (!(ok = mbar_wait(full_bar(s), ph, abort_flag, a.timeout_ns, a.err, 43))) break;
+      constexpr uint32_t idesc = make_idesc(128, TN, 0);  // e4m3 operands, fp32 accumulator
+      const uint32_t leader = elect_one();
+      const uint32_t q0 = smem_u32(smem) + L.q, d0 = smem_u32(smem) + L.stage;
+      int s = 0;
+      uint32_t ph = 0, u = 0;
+      bool ok = true;
+      for (int t = 0; ok && t < n_tiles; ++t) {
+        ok = mbar_wait(full_bar(s), ph, abort_flag, a.timeout_ns, a.err, 43);
+        ok = __all_sync(kAllWarp, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t b0 = d0 + static_cast<uint32_t>(s) * L.stage_bytes;
+        for (int m = 0; m < mt; ++m, ++u) {
+          const uint32_t slot = u % kSlots;
+          ok = mbar_wait(acce_bar(slot), ((u / kSlots) & 1u) ^ 1u, abort_flag, a.timeout_ns, a.err, 44);
+          ok = __all_sync(kAllWarp, ok);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t b0 = smem_u32(smem) + L.stage + static_cast<uint32_t>(s) * L.stage_bytes;
-          for (int m = 0; ok && m < mt; ++m, ++u) {
-            const uint32_t slot = u % kSlots;
-            if (!(ok = mbar_wait(acce_bar(slot), ((u / kSlots) & 1u) ^ 1u, abort_flag, a.timeout_ns, a.err, 44))) break;
-            tc_fence_after();
-            uint32_t acc = 0;
-            for (int term = 0; term < a.terms; ++term)
-              for (int c = 0; c < a.kc; ++c) {
-                const int left = a.d - c * 128;
-                const int steps = left >= 128 ? 4 : (left + 31) / 32;
-                const uint64_t ad = sw128_kmajor_desc(
-                    smem_u32(smem) + L.q + static_cast<uint32_t>((m * a.terms + term) * a.kc + c) * kChunkTile);
-                const uint64_t bd = sw128_kmajor_desc(b0 + static_cast<uint32_t>(c * TN * 128));
-                for (int k = 0; k < steps; ++k) {
-                  mma_f8(tmem + slot * TN, ad + 2 * k, bd + 2 * k, idesc, acc);
-                  acc = 1;
-                }
+          uint32_t acc = 0;
+          for (int term = 0; term < a.terms; ++term)
+            for (int c = 0; c < a.kc; ++c) {
+              const int left = a.d - c * 128;
+              const uint64_t ad = sw128_kmajor_desc(q0 + static_cast<uint32_t>((m * a.terms + term) * a.kc + c) * kChunkTile);
+              const uint64_t bd = sw128_kmajor_desc(b0 + static_cast<uint32_t>(c * TN * 128));
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (k * 32 >= left) break;
+                mma_f8(tmem + slot * TN, ad + 2 * k, bd + 2 * k, idesc, acc, leader);
+                acc = 1;
               }
-            mma_commit(accf_bar(slot));
-          }
-          if (ok) mma_commit(empty_bar(s));
-          if (++s == a.stages) { s = 0; ph ^= 1u; }
+            }
+          commit(accf_bar(slot), leader);
         }
-        mma_commit(done_bar);  // nothing is in flight when the CTA ends
-        mbar_wait(done_bar, 0, never_flag, a.timeout_ns, a.err, 45);
+        if (ok) commit(empty_bar(s), leader);
+        if (++s == a.stages) { s = 0; ph ^= 1u; }
       }
+      commit(done_bar, leader);  // nothing is in flight when the CTA ends
+      mbar_wait(done_bar, 0, never_flag, a.timeout_ns, a.err, 45);
     } else {
       // ---------------------------------------------------------------- epilogue
       const int quarter = warp & 3, half = (warp - kEpiWarp0) >> 2;
