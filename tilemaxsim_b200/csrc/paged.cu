@@ -8,6 +8,8 @@
 // maximum over the document's tokens and no reader needs the lengths.
 //
 // No counterpart in the reference, whose corpora are fixed tensors (src/flash_maxsim_kernel.py:248-273).
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -200,6 +202,18 @@ __global__ void __launch_bounds__(kTableThreads) table_fill_kernel(const TableAr
 // ------------------------------------------------------------------------------------------------
 constexpr float kE4m3Max = 448.f;
 
+// Four fp32 values as e4m3, to nearest, ties to even; larger magnitudes give 448, a NaN 0x7f.
+__device__ __forceinline__ uint32_t e4m3x4(float2 lo, float2 hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 p, q;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 p, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 q, %4, %3;\n\t"
+      "mov.b32 %0, {p, q};\n\t}\n"
+      : "=r"(r)
+      : "f"(lo.x), "f"(lo.y), "f"(hi.x), "f"(hi.y));
+  return r;
+}
+
 struct WriteArgs {
   const void* x;
   const void* residual;  // nullptr, or laid out as x
@@ -221,21 +235,6 @@ struct WriteArgs {
   int64_t n_pages;
 };
 
-// Eight consecutive elements of a row.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
-    v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(e[i]);
-  }
-}
-
 __device__ __forceinline__ bool finite(double v) { return fabs(v) <= 1.7e308; }
 
 // e4m3 of a double, rounded once: to odd on the way to fp32 (24 bits, more than e4m3's 4 + 2), then
@@ -243,130 +242,444 @@ __device__ __forceinline__ bool finite(double v) { return fabs(v) <= 1.7e308; }
 __device__ __forceinline__ uint8_t e4m3_of_double(double t) {
   float f = __double2float_rz(t);
   if (static_cast<double>(f) != t) f = __uint_as_float(__float_as_uint(f) | 1u);
-  return static_cast<uint8_t>(__nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3));
+  return static_cast<uint8_t>(e4m3x4(make_float2(f, 0.f), make_float2(0.f, 0.f)) & 0xffu);
 }
 
-constexpr int kWriteThreads = 128;
-
-// One CTA a page. Pass one: each row's sum of squares and largest magnitude, then the page's
-// largest normalised magnitude and its scale. Pass two: the codes. A group of lanes holds a row,
-// eight elements a lane.
+// Eight consecutive elements of a row, as they are stored.
 template <typename T>
-__global__ void __launch_bounds__(kWriteThreads) page_write_kernel(const WriteArgs a) {
-  __shared__ double row_factor[128];
-  __shared__ double warp_max[kWriteThreads / 32];
-  __shared__ int bad_any;
+struct Eight {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void take(const T* p) {  // from shared memory
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = make_uint4(0, 0, 0, 0);
+  }
+  // The largest magnitude of 16-bit values, two at a time: their bits without the sign are ordered
+  // as they are (a NaN's above infinity's).
+  __device__ __forceinline__ float top() const {
+    const uint32_t m = __vmaxu2(__vmaxu2(v[0].x & 0x7fff7fffu, v[0].y & 0x7fff7fffu),
+                                __vmaxu2(v[0].z & 0x7fff7fffu, v[0].w & 0x7fff7fffu));
+    const uint32_t w = max(m & 0xffffu, m >> 16);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(w << 16);
+    else return __half2float(__ushort_as_half(static_cast<unsigned short>(w)));
+  }
+  __device__ __forceinline__ float at(int i) const {
+    const uint4& q = v[sizeof(T) == 4 ? i >> 2 : 0];
+    const int j = sizeof(T) == 4 ? i & 3 : i >> 1;
+    const uint32_t w = j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w;
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    else
+      return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w >> 16 : w)));
+  }
+};
+
+// One page at a time a CTA of four warps, the next page on its way into shared memory (cp.async)
+// meanwhile; a group of 2 to 32 lanes takes a row, eight elements a lane. The input is read from
+// memory once and the codes are written once, which bounds the kernel. Pages of more than
+// kStageBytes of input are read twice instead, the second time from the caches.
+//
+// The scale is the fp32 rounding, and every code the e4m3 rounding, of what 64 bits give, at little
+// more than fp32's cost. fp32 gives every row's factor to 2^-21. Only rows whose largest magnitude
+// comes within 2^-19 of the page's can set the scale: they (one, as a rule) are summed again in
+// fp64. A code is that of t = h * w * factor / scale: where t * (1 - 2^-20) and t * (1 + 2^-20)
+// round to the same one, fp32 is sure of it; the others (about one of 4,000 groups of eight
+// elements) are done again in fp64. Pages that hold a magnitude or a sum of squares outside [1e-30,
+// 1e30], zeros apart, go through fp64 altogether; NaN and infinities are found there.
+//
+// 20,000 documents (3.6M tokens, 128 bf16 values, unit length), in us: rows held in registers, all
+// sums in fp64 600-820, in fp32 770 (few warps fit); see the launch for what this form takes.
+__device__ __forceinline__ double max_keep_nan(double x, double y) { return y <= x || x != x ? x : y; }
+__device__ __forceinline__ bool usual(float v) { return v >= 1e-30f && v <= 1e30f; }
+
+#ifndef WT
+#define WT 64
+#endif
+constexpr int kWriteThreads = WT;
+constexpr int kStageBytes = 24 * 1024;  // most input of a page (x and residual) that is staged
+
+struct Entry {    // where a table entry's rows come from
+  int64_t at;     // element offset of its first row
+  int64_t id;
+  int limit;      // rows of x from there on, up to a page
+  int count;      // 0: the entry is skipped
+};
+
+template <typename T, bool SUM, bool WEIGHT, bool STAGED>
+struct PageRows {
+  const WriteArgs& a;
+  const T* stage;  // x's rows, then the residual's
+  int sub, group;
+  bool in_row;
+  // Eight elements of row src (of the page) of x, and of the residual.
+  __device__ __forceinline__ void load(const Entry& e, int src, Eight<T>& x, Eight<T>& r) const {
+    if (!in_row || (!STAGED && src >= e.limit)) {
+      x.zero();
+      if constexpr (SUM) r.zero();
+      return;
+    }
+    if constexpr (STAGED) {
+      const T* const p = stage + src * a.d + sub * 8;
+      x.take(p);
+      if constexpr (SUM) r.take(p + (a.d << a.page_shift));
+    } else {
+      const int64_t at = e.at + src * a.stride_tok + sub * 8;
+      x.load(static_cast<const T*>(a.x) + at);
+      if constexpr (SUM) r.load(static_cast<const T*>(a.residual) + at);
+    }
+  }
+};
+
+// A row in fp64, by the lanes that hold it: its eight elements a lane (times the weights), its
+// largest magnitude before the factor, and its factor: from fp32's one by a Newton step, which
+// squares its 2^-21, or, where `full`, by fp64's own root and quotient.
+struct ExactRow {
+  double h[8], factor, top;
+  bool bad;
+};
+template <typename T, bool SUM, bool WEIGHT, bool STAGED>
+__device__ __forceinline__ void exact_row(const PageRows<T, SUM, WEIGHT, STAGED>& rows, const Entry& e, int src,
+                                          float near, bool full, ExactRow& o) {
+  const WriteArgs& a = rows.a;
+  Eight<T> x, r;
+  rows.load(e, src, x, r);
+  double s = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    o.h[j] = x.at(j);
+    if constexpr (SUM) o.h[j] += static_cast<double>(r.at(j));
+    s = fma(o.h[j], o.h[j], s);
+  }
+  if constexpr (WEIGHT) {
+    Eight<T> w;
+    w.zero();
+    if (rows.in_row) w.load(static_cast<const T*>(a.weight) + rows.sub * 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o.h[j] *= static_cast<double>(w.at(j));
+  }
+  for (int m = rows.group >> 1; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+  o.top = 0.0;
+  if (SUM || (WEIGHT && sizeof(T) == 4) || full) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o.top = max_keep_nan(o.top, fabs(o.h[j]));
+    for (int m = rows.group >> 1; m > 0; m >>= 1) o.top = max_keep_nan(o.top, __shfl_xor_sync(0xffffffffu, o.top, m));
+  } else {  // the magnitudes are exact in fp32
+    float top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(static_cast<float>(o.h[j])));
+    for (int m = rows.group >> 1; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+    o.top = top;
+  }
+  o.factor = 1.0;
+  o.bad = false;
+  if (!full) {
+    const double f = near, v = a.norm == TMS_NORM_RMS ? s * (1.0 / a.d) + a.eps : s;
+    if (a.norm != TMS_NORM_NONE) o.factor = f + 0.5 * f * (1.0 - v * f * f);
+    return;
+  }
+  if (a.norm == TMS_NORM_L2) {
+    const double n = sqrt(s);
+    o.factor = 1.0 / (n > a.eps ? n : static_cast<double>(a.eps));
+  } else if (a.norm == TMS_NORM_RMS) {
+    o.factor = 1.0 / sqrt(s / a.d + a.eps);
+  }
+  o.bad = !(finite(s) && finite(o.top * o.factor));
+}
+
+template <typename T, bool SUM, bool WEIGHT, bool STAGED>
+__global__ void __launch_bounds__(kWriteThreads, 1024 / kWriteThreads) page_write_kernel(const WriteArgs a, int group) {
+  constexpr uint32_t kAllWarp = 0xffffffffu;
+  constexpr int kWarps = kWriteThreads / 32;
+  extern __shared__ __align__(16) uint8_t stage_bytes[];
+  __shared__ Entry entries[3];
+  __shared__ float row_factor[128], row_top[128];
+  __shared__ float warp_top[kWarps];
+  __shared__ double warp_best[kWarps];
+  __shared__ int warp_odd[kWarps], warp_bad[kWarps];
   const int page = 1 << a.page_shift;
-  const int vecs = a.d >> 3;
-  int group = 2;  // lanes of a row: a power of two, at most 32
-  while (group < vecs) group <<= 1;
-  const int sub = threadIdx.x % group, row0 = threadIdx.x / group, rows_step = kWriteThreads / group;
-  const bool in_row = sub < vecs;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = threadIdx.x & (group - 1), step = kWriteThreads / group, row0 = threadIdx.x / group;
+  const bool in_row = sub < (a.d >> 3);
+  T* const stages = reinterpret_cast<T*>(stage_bytes);
+  const int stage_elems = (a.d << a.page_shift) * (SUM ? 2 : 1);
+  Eight<T> wt;
+  wt.zero();
+  bool odd_weight = false;
+  if (WEIGHT && in_row) {
+    wt.load(static_cast<const T*>(a.weight) + sub * 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) odd_weight |= !(fabsf(wt.at(j)) <= 1e30f);
+  }
+  const float per_d = 1.f / a.d;
+  // After the sums below a lane has those of `held` of its four rows, from row number `mine` on.
+  const int held = group == 2 ? 2 : 1;
+  const int mine = group == 2 ? (sub & 1) * 2 : (sub & 1) * 2 + (sub >> 1 & 1);
+
   const int64_t total_all = a.page_offsets[a.n_docs];
   const int64_t total = total_all < a.page_cap ? total_all : a.page_cap;
-  double w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = 1.0;
-  if (a.weight && in_row) {
-    float wf[8];
-    load8(static_cast<const T*>(a.weight) + sub * 8, wf);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = wf[i];
-  }
-  for (int64_t k = blockIdx.x; k < total; k += gridDim.x) {
-    const int64_t doc = a.page_docs[k], id = a.page_ids[k];
-    if (doc < 0 || doc >= a.n_docs || id < 0 || id >= a.n_pages) continue;
-    const int64_t nth = k - a.page_offsets[doc];
-    const int64_t t0 = a.token_offsets[doc];
-    if (nth < 0 || nth > k || t0 < 0 || (!a.padded && t0 > a.n_rows)) continue;  // malformed tables
+  auto find = [&](int64_t k) {
+    Entry e = {0, 0, 0, 0};
+    if (k >= total) return e;
+    const int64_t doc = __ldg(a.page_docs + k);
+    e.id = __ldg(a.page_ids + k);
+    if (doc < 0 || doc >= a.n_docs || e.id < 0 || e.id >= a.n_pages) return e;
+    const int64_t nth = k - __ldg(a.page_offsets + doc);
+    const int64_t t0 = __ldg(a.token_offsets + doc), t1 = __ldg(a.token_offsets + doc + 1);
+    if (nth < 0 || nth > k || t0 < 0 || (!a.padded && t0 > a.n_rows)) return e;  // malformed tables
     const int64_t first = nth << a.page_shift;
-    const int64_t left = a.token_offsets[doc + 1] - t0 - first;
-    if (left < 1) continue;
-    const int count = left < page ? static_cast<int>(left) : page;
-    // rows [first, first + count) of the document; rows outside x read as zeros
-    const int64_t doc_off = a.padded ? doc * a.stride_doc : t0 * a.stride_tok;
+    const int64_t left = t1 - t0 - first;
     const int64_t limit = a.padded ? a.n_rows - first : a.n_rows - t0 - first;
-    const T* const x = static_cast<const T*>(a.x) + doc_off + first * a.stride_tok;
-    const T* const res =
-        a.residual ? static_cast<const T*>(a.residual) + doc_off + first * a.stride_tok : nullptr;
-    auto load = [&](int r, double (&h)[8]) {
-      float v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = 0.0;
-      if (!in_row || r >= limit) return;
-      load8(x + r * a.stride_tok + sub * 8, v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = v[i];
-      if (res) {
-        load8(res + r * a.stride_tok + sub * 8, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] += v[i];
-      }
-    };
-    if (threadIdx.x == 0) bad_any = 0;
-    __syncthreads();
-    double best = 0.0;
-    bool bad = false;
-    for (int r0 = 0; r0 < page; r0 += rows_step) {
-      const int r = r0 + row0;
-      double h[8], s = 0.0, m = 0.0;
-      const bool on = r < count;
-      if (on) load(r, h);
+    e.at = (a.padded ? doc * a.stride_doc : t0 * a.stride_tok) + first * a.stride_tok;
+    e.limit = limit < 0 ? 0 : limit < page ? static_cast<int>(limit) : page;
+    e.count = left < 1 ? 0 : left < page ? static_cast<int>(left) : page;
+    return e;
+  };
+  // This thread's part of every row it takes: the same lanes copy a row that read it.
+  const int64_t row_jump = step * a.stride_tok, my_from = row0 * a.stride_tok + sub * 8;
+  const uint32_t my_to = smem_u32(stage_bytes) + (row0 * a.d + sub * 8) * static_cast<uint32_t>(sizeof(T));
+  const uint32_t to_jump = step * a.d * static_cast<uint32_t>(sizeof(T));
+  auto fetch = [&](const Entry& e, int which) {  // the entry's rows into a stage
+    const int count = e.count < e.limit ? e.count : e.limit;
+    uint32_t to = my_to + which * stage_elems * static_cast<uint32_t>(sizeof(T));
+    const T* from = static_cast<const T*>(a.x) + e.at + my_from;
+    const T* from_res = static_cast<const T*>(a.residual) + e.at + my_from;
+    const uint32_t res = (a.d << a.page_shift) * static_cast<uint32_t>(sizeof(T));
+    if (!in_row) return;
+    for (int row = row0 + (count - row0 + step - 1) / step * step; row < e.count; row += step) {  // rows x does not have
+      if (row < count) continue;
+      T* const p = stages + which * stage_elems + row * a.d + sub * 8;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (!on) h[i] = 0.0;
-        s += h[i] * h[i];
-        const double y = fabs(h[i] * w[i]);
-        if (!(y <= m) && m == m) m = y;  // a NaN stays
+        p[i] = T(0.f);
+        if constexpr (SUM) p[(a.d << a.page_shift) + i] = T(0.f);
       }
-      for (int o = group >> 1; o > 0; o >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, o);
-        const double y = __shfl_xor_sync(0xffffffffu, m, o);
-        if (!(y <= m) && m == m) m = y;
+    }
+    for (int row = row0; row < count; row += step, to += to_jump, from += row_jump) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) cp_async16(to + 16 * i, from + i * (16 / sizeof(T)));
+      if constexpr (SUM) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+          cp_async16(to + res + 16 * i, from_res + i * (16 / sizeof(T)));
+        from_res += row_jump;
       }
-      double f = 1.0;
-      if (a.norm == TMS_NORM_L2) {
-        const double n = sqrt(s);
-        f = 1.0 / (n > a.eps ? n : static_cast<double>(a.eps));
-      } else if (a.norm == TMS_NORM_RMS) {
-        f = 1.0 / sqrt(s / a.d + a.eps);
+    }
+  };
+
+  if (threadIdx.x == 0) entries[0] = find(blockIdx.x);
+  __syncthreads();
+  if constexpr (STAGED) fetch(entries[0], 0);
+  int now = 0, at = 0;  // the stage, and the place among the entries, of this page
+  for (int64_t k = blockIdx.x; k < total; k += gridDim.x, now ^= 1, at = at == 2 ? 0 : at + 1) {
+    const int after = at == 2 ? 0 : at + 1;
+    if (threadIdx.x == 0) entries[after] = find(k + gridDim.x);
+    if constexpr (STAGED) cp_async_wait_all();
+    __syncthreads();  // this page's rows are there, the next entry is known, the page before is done
+    if constexpr (STAGED) fetch(entries[after], now ^ 1);
+    const Entry e = entries[at];
+    if (e.count == 0) continue;  // the same for the whole CTA
+    const PageRows<T, SUM, WEIGHT, STAGED> rows{a, stages + now * stage_elems, sub, group, in_row};
+
+    float top = 0.f;
+    bool odd = odd_weight;
+    for (int r0 = row0, b = 0; b < page; r0 += 4 * step, b += 4 * step) {  // the same turns for all lanes
+      float sums[4], tops[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sums[i] = tops[i] = 0.f;
+        const int row = r0 + i * step;
+        if (row >= e.count) continue;
+        Eight<T> x, r;
+        rows.load(e, row, x, r);
+        uint64_t s2 = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          float h0 = x.at(j), h1 = x.at(j + 1);
+          if constexpr (SUM) h0 += r.at(j), h1 += r.at(j + 1);
+          const uint64_t h2 = f2_pack(h0, h1);
+          s2 = f2_fma(h2, h2, s2);
+          if constexpr (SUM || WEIGHT || sizeof(T) == 4) {
+            if constexpr (WEIGHT) h0 *= wt.at(j), h1 *= wt.at(j + 1);
+            tops[i] = fmaxf(tops[i], fmaxf(fabsf(h0), fabsf(h1)));  // a NaN shows in the sum
+          }
+        }
+        const float2 two = f2_unpack(s2);
+        sums[i] = two.x + two.y;
+        if constexpr (!(SUM || WEIGHT || sizeof(T) == 4)) tops[i] = x.top();
       }
-      if (on && sub == 0) row_factor[r] = f;
-      const double y = m * f;
-      bad |= on && !(finite(s) && finite(y));
-      if (on && y > best) best = y;
+      // Over the lanes of a group: while a lane has more than one row, it hands half of them to its
+      // partner and takes the other half's partial results; then plain exchanges.
+      {
+        const bool upper = sub & 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float s = __shfl_xor_sync(kAllWarp, upper ? sums[i] : sums[i + 2], 1);
+          const float t = __shfl_xor_sync(kAllWarp, upper ? tops[i] : tops[i + 2], 1);
+          sums[i] = (upper ? sums[i + 2] : sums[i]) + s;
+          tops[i] = fmaxf(upper ? tops[i + 2] : tops[i], t);
+        }
+      }
+      if (group > 2) {
+        const bool upper = sub & 2;
+        const float s = __shfl_xor_sync(kAllWarp, upper ? sums[0] : sums[1], 2);
+        const float t = __shfl_xor_sync(kAllWarp, upper ? tops[0] : tops[1], 2);
+        sums[0] = (upper ? sums[1] : sums[0]) + s;
+        tops[0] = fmaxf(upper ? tops[1] : tops[0], t);
+        for (int o = 4; o < group; o <<= 1) {
+          sums[0] += __shfl_xor_sync(kAllWarp, sums[0], o);
+          tops[0] = fmaxf(tops[0], __shfl_xor_sync(kAllWarp, tops[0], o));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = r0 + (mine + i) * step;
+        if (i >= held || row >= e.count) break;
+        float f = 1.f;
+        odd |= !((usual(tops[i]) || (WEIGHT && tops[i] == 0.f)) && usual(sums[i])) && !(sums[i] == 0.f && tops[i] == 0.f);
+        if (a.norm != TMS_NORM_NONE) {
+          if (a.norm == TMS_NORM_L2) {
+            f = sums[i] > 0.f ? rsqrtf(sums[i]) : 1.f;
+            odd |= sums[i] > 0.f && !(f * a.eps < 0.999f);  // at or under eps
+          } else {
+            f = rsqrtf(fmaf(sums[i], per_d, a.eps));
+          }
+          odd |= !usual(f);
+        }
+        const float t = tops[i] * f;
+        row_factor[row] = f;
+        row_top[row] = t;
+        top = fmaxf(top, t);
+      }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double y = __shfl_xor_sync(0xffffffffu, best, o);
-      if (y > best) best = y;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAllWarp, top, o));
+    odd = __any_sync(kAllWarp, odd);
+    if (lane == 0) {
+      warp_top[warp] = top;
+      warp_odd[warp] = odd;
     }
-    if (lane_id() == 0) warp_max[threadIdx.x >> 5] = best;
-    if (bad) bad_any = 1;
     __syncthreads();
-    best = warp_max[0];
-    for (int i = 1; i < kWriteThreads / 32; ++i)
-      if (warp_max[i] > best) best = warp_max[i];
-    const bool poison = bad_any != 0;
-    const float scale = poison ? __int_as_float(0x7fffffff) : static_cast<float>(best / kE4m3Max);
-    for (int r0 = 0; r0 < page; r0 += rows_step) {
-      const int r = r0 + row0;
-      const int src = r < count ? r : count - 1;
-      if (r < page && in_row) {
-        double h[8];
-        load(src, h);
-        const double f = row_factor[src];
-        alignas(8) uint8_t c[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          c[i] = poison ? 0x7f : scale > 0.f ? e4m3_of_double(h[i] * w[i] * f / scale) : 0;
-        *reinterpret_cast<uint2*>(a.codes + ((id << a.page_shift) + r) * a.d + sub * 8) =
-            *reinterpret_cast<const uint2*>(c);
+    for (int i = 0; i < kWarps; ++i) {
+      top = fmaxf(top, warp_top[i]);
+      odd |= warp_odd[i] != 0;
+    }
+    // Rows that can set the scale, a warp for each 32 rows.
+    double best = 0.0;
+    bool bad = false;
+    for (int base = warp * 32; base < page; base += kWriteThreads) {
+      const int row = base + lane;
+      uint32_t might = __ballot_sync(kAllWarp, row < e.count && (odd || row_top[row] >= top * (1.f - 0x1p-19f)));
+      while (might) {
+        const int r = base + __ffs(might) - 1;
+        might &= might - 1;
+        ExactRow exact;
+        exact_row(rows, e, r, row_factor[r], odd, exact);
+        bad |= exact.bad;
+        const double y = exact.top * exact.factor;
+        if (y > best) best = y;
       }
     }
-    if (threadIdx.x == 0) a.scales[id] = scale;
+    if (lane == 0) {
+      warp_best[warp] = best;
+      warp_bad[warp] = bad;
+    }
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      if (warp_best[i] > best) best = warp_best[i];
+      bad |= warp_bad[i] != 0;
+    }
+    const float scale = bad ? __int_as_float(0x7fffffff) : static_cast<float>(best * (1.0 / kE4m3Max));
+    const bool plain = !odd && usual(scale);
+    const float inverse = __frcp_rn(scale);
+    if (threadIdx.x == 0) a.scales[e.id] = scale;
+    uint8_t* const out = a.codes + (e.id << a.page_shift) * a.d + sub * 8;
+    for (int r0 = row0, b = 0; b < page; r0 += 4 * step, b += 4 * step) {  // the same turns for all lanes
+      uint32_t unsure = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = r0 + i * step;
+        if (row >= page) break;
+        const int src = row < e.count ? row : e.count - 1;  // behind the last token: that token again
+        Eight<T> x, r;
+        rows.load(e, src, x, r);
+        const float g = row_factor[src] * inverse;
+        const float under = g * (1.f - 0x1p-20f), over = g * (1.f + 0x1p-20f);
+        uint32_t word[2], other[2];
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          float h[4];
+#pragma unroll
+          for (int l = 0; l < 4; ++l) {
+            h[l] = x.at(j + l);
+            if constexpr (SUM) h[l] += r.at(j + l);
+            if constexpr (WEIGHT) h[l] *= wt.at(j + l);
+          }
+          const uint64_t p0 = f2_pack(h[0], h[1]), p1 = f2_pack(h[2], h[3]);
+          const uint64_t lo2 = f2_pack(under, under), hi2 = f2_pack(over, over);
+          word[j >> 2] = e4m3x4(f2_unpack(f2_mul(p0, lo2)), f2_unpack(f2_mul(p1, lo2)));
+          other[j >> 2] = e4m3x4(f2_unpack(f2_mul(p0, hi2)), f2_unpack(f2_mul(p1, hi2)));
+        }
+        if (!plain || !usual(g) || ((word[0] ^ other[0]) | (word[1] ^ other[1]))) unsure |= 1u << i;
+        if (in_row) *reinterpret_cast<uint2*>(out + row * a.d) = make_uint2(word[0], word[1]);
+      }
+      // Rows that fp32 is not sure of, again.
+      uint32_t again = __reduce_or_sync(kAllWarp, unsure);
+      while (again) {
+        const int i = __ffs(again) - 1;
+        again &= again - 1;
+        const int row = r0 + i * step;
+        const int src = row < e.count ? row : e.count - 1;
+        ExactRow exact;
+        exact_row(rows, e, src, row_factor[src], !plain, exact);
+        if (!(unsure >> i & 1u) || row >= page || !in_row) continue;
+        const double inv = inverse;
+        const double gain = exact.factor * (inv + inv * (1.0 - inv * scale));  // used where plain
+        uint32_t word[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t code = bad ? 0x7fu : scale > 0.f ? e4m3_of_double(plain ? exact.h[j] * gain : exact.h[j] * exact.factor / scale) : 0u;
+          word[j >> 2] |= code << (8 * (j & 3));
+        }
+        *reinterpret_cast<uint2*>(out + row * a.d) = make_uint2(word[0], word[1]);
+      }
+    }
   }
+  if constexpr (STAGED) cp_async_wait_all();
+}
+
+template <typename T, bool SUM, bool WEIGHT>
+cudaError_t launch_write_as(const WriteArgs& a, const DeviceInfo* dev, cudaStream_t st) {
+  int group = 2;  // lanes of a row
+  while (group * 8 < a.d) group <<= 1;
+  const int input = (a.d << a.page_shift) * static_cast<int>(sizeof(T)) * (SUM ? 2 : 1);
+  const bool staged = input <= kStageBytes;
+  const int64_t most = static_cast<int64_t>(dev->num_sms) * 12;
+  const unsigned blocks = static_cast<unsigned>(a.page_cap < most ? a.page_cap : most);
+  if (staged) {
+    auto kern = page_write_kernel<T, SUM, WEIGHT, true>;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStageBytes);
+    if (e != cudaSuccess) return e;
+    kern<<<blocks, kWriteThreads, 2 * input, st>>>(a, group);
+  } else {
+    page_write_kernel<T, SUM, WEIGHT, false><<<blocks, kWriteThreads, 0, st>>>(a, group);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_write(const WriteArgs& a, const DeviceInfo* dev, cudaStream_t st) {
+  if (a.residual) return a.weight ? launch_write_as<T, true, true>(a, dev, st) : launch_write_as<T, true, false>(a, dev, st);
+  return a.weight ? launch_write_as<T, false, true>(a, dev, st) : launch_write_as<T, false, false>(a, dev, st);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -496,13 +809,10 @@ extern "C" int tms_page_write(const void* x, int dtype, int64_t n_rows, int64_t 
   const WriteArgs a{x, residual, weight, stride_doc, stride_token, n_rows, padded, norm, eps,
                     static_cast<int>(d), shift, page_offsets, token_offsets, page_ids, page_docs, n_docs,
                     page_capacity, static_cast<uint8_t*>(codes), scales, n_pages};
-  const int64_t most = static_cast<int64_t>(dev->num_sms) * 12;
-  const unsigned blocks = static_cast<unsigned>(page_capacity < most ? page_capacity : most);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == TMS_F16) page_write_kernel<__half><<<blocks, kWriteThreads, 0, st>>>(a);
-  else if (dtype == TMS_BF16) page_write_kernel<__nv_bfloat16><<<blocks, kWriteThreads, 0, st>>>(a);
-  else page_write_kernel<float><<<blocks, kWriteThreads, 0, st>>>(a);
-  return cuda_status(cudaGetLastError());
+  return cuda_status(dtype == TMS_F16    ? launch_write<__half>(a, dev, st)
+                     : dtype == TMS_BF16 ? launch_write<__nv_bfloat16>(a, dev, st)
+                                         : launch_write<float>(a, dev, st));
 }
 
 extern "C" int tms_page_read(const void* codes, const float* scales, int64_t n_pages,

@@ -399,8 +399,19 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
   }
   n_tiles = uniform(n_tiles);
 
-  if (dead || n_tiles == 0) {
-    // no role runs (misaligned shared memory, or nothing to score)
+  // Documents without a table entry: this CTA's share of them, done by the epilogue warps while the
+  // first tile is on its way.
+  auto write_empty = [&]() {
+    const int64_t lo = a.n_docs * range / a.ranges, hi = a.n_docs * (range + 1) / a.ranges;
+    for (int64_t doc = lo + threadIdx.x - kEpiWarp0 * 32; doc < hi; doc += kThreads - kEpiWarp0 * 32) {
+      if (clamp_entry(a, __ldg(a.page_offsets + doc)) < clamp_entry(a, __ldg(a.page_offsets + doc + 1))) continue;
+      for (int c = m_first * 4; c < (m_first + mt) * 4 && c < a.n_chunks; ++c) a.out[c * a.n_docs + doc] = kNegInf;
+    }
+  };
+  if (dead) {
+    // no role runs: misaligned shared memory
+  } else if (n_tiles == 0) {
+    if (warp >= kEpiWarp0) write_empty();
   } else if (warp == 0) {
     // ------------------------------------------------------------------ loads: a lane for each box
     static_assert(kTile / U <= 32, "a lane for each box");
@@ -411,14 +422,22 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
     auto page_of = [&](int unit) -> int64_t {
       return unit < mine.units ? __ldg(a.page_ids + mine.first + (unit >> a.unit_shift)) : -1;
     };
-    int64_t next = page_of(nth);
+    // Page ids are fetched kAhead tiles ahead: one tile ahead, the wait for them paced the loop.
+    constexpr int kAhead = 4;
+    int64_t ids[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ids[i] = page_of(i * kUnits + nth);
     int s = 0;
     uint32_t ph = 0, armed = 0, armed_par = 0;
     bool ok = !(a.debug_flags & 1);
-    for (int t = 0; ok && t < n_tiles; ++t) {
+    for (int t0 = 0; ok && t0 < n_tiles; t0 += kAhead) {
+#pragma unroll
+     for (int i = 0; i < kAhead; ++i) {
+      const int t = t0 + i;
+      if (!ok || t >= n_tiles) break;
       const int unit = t * kUnits + nth;
-      const int64_t id = next;
-      if (t + 1 < n_tiles) next = page_of(unit + kUnits);
+      const int64_t id = ids[i];
+      ids[i] = page_of(unit + kAhead * kUnits);
       const bool load = id >= 0 && id < a.n_pages;
       const uint32_t boxes = __popc(__ballot_sync(kAllWarp, load));
       const int32_t y = static_cast<int32_t>(id << a.page_shift) + (unit & half_mask) * U;
@@ -435,6 +454,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
                       full_bar(s), c * 128, y, policy);
         if (++s == a.stages) { s = 0; ph ^= 1u; }
       }
+     }
     }
     // every copy lands before the CTA ends, also where a wait of another role gave up
     for (int i = 0; i < a.stages; ++i)
@@ -530,6 +550,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       // scale (-1: no page there) and the document that ends with the box (-1: none does).
       float cur_scale = 0.f, next_scale = 0.f;
       int cur_ends = -1, next_ends = -1;
+      uint32_t end_mask = 0;  // a bit for each of the 32 boxes with which a document ends
       auto fetch = [&](int u0) {
         const int u = u0 + lane;
         next_scale = -1.f;
@@ -545,6 +566,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
         }
       };
       fetch(0);
+      write_empty();
       for (int m = 0; m < mt; ++m) bests[m * 32] = kNegInf;
       bool open = streams[stream].open;  // the document in hand began in the stream before
       if (lane == 0) head_docs[me] = -1;
@@ -556,8 +578,13 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
         if ((unit0 & 31) == 0) {
           cur_scale = next_scale;
           cur_ends = next_ends;
+          end_mask = __ballot_sync(kAllWarp, cur_ends >= 0);
           fetch(unit0 + 32);  // also past the stream's end: another stream may go on
         }
+        float scales[kUnits];
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) scales[i] = __shfl_sync(kAllWarp, cur_scale, (unit0 + i) & 31);
+        const uint32_t ends_here = end_mask >> (unit0 & 31);
         bool still_open = open;
         for (int m = 0; m < mt; ++m) {
           float best = bests[m * 32];
@@ -567,11 +594,9 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
           const uint32_t at = tmem + slot * kCols + half * W + (static_cast<uint32_t>(quarter * 32) << 16);
           still_open = open;
           auto one = [&](int i, float v) {  // box i of the tile is done
-            const int from = (unit0 + i) & 31;
-            const float scale = __shfl_sync(kAllWarp, cur_scale, from);
-            const int ends = __shfl_sync(kAllWarp, cur_ends, from);
-            if (!(scale < 0.f)) best = max_nan(best, v * scale);
-            if (ends >= 0) {
+            if (!(scales[i] < 0.f)) best = max_nan(best, v * scales[i]);
+            if (ends_here >> i & 1u) {
+              const int ends = __shfl_sync(kAllWarp, cur_ends, (unit0 + i) & 31);
               if (still_open) {  // joined with the streams before at the end
                 heads[m * 32] = best;
                 if (lane == 0) head_docs[me] = ends;
@@ -633,13 +658,6 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       }
       if (queued) flush();
     }
-  }
-
-  // Documents without a table entry: this CTA's share of them.
-  const int64_t lo = a.n_docs * range / a.ranges, hi = a.n_docs * (range + 1) / a.ranges;
-  for (int64_t doc = lo + threadIdx.x; doc < hi; doc += kThreads) {
-    if (clamp_entry(a, __ldg(a.page_offsets + doc)) < clamp_entry(a, __ldg(a.page_offsets + doc + 1))) continue;
-    for (int c = m_first * 4; c < (m_first + mt) * 4 && c < a.n_chunks; ++c) a.out[c * a.n_docs + doc] = kNegInf;
   }
 
   tc_fence_before();
