@@ -263,7 +263,7 @@ TMS_API int tms_topk_merge_packed(const int64_t* gathered, int64_t world, int64_
  * token. d is a multiple of 16, at most TMS_PAGED_MAX_D. Whatever the tables hold, no call reads or
  * writes outside its arrays: an entry whose page id lies outside the pool is skipped. */
 
-TMS_API size_t tms_page_tables_workspace_size(int64_t n_docs);
+TMS_API size_t tms_page_tables_workspace_size(int64_t n_docs, int64_t page_capacity);
 
 /* The page tables and token slots of n_docs documents, from their lengths. Document i's length is
  * lengths[i], or lengths[doc_ids[i]] when doc_ids != NULL (an id outside [0, n_lengths) and a

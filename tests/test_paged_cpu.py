@@ -99,8 +99,8 @@ def test_c_abi_refusals_without_gpu():
     p = ctypes.c_void_p(1 << 20)  # an aligned address that is never read: every call below is refused or empty
     odd = ctypes.c_void_p((1 << 20) + 8)
 
-    def tables(lengths=p, n=2, page=32, po=p, ids=p, cap=4, ws=p, wsb=1 << 20):
-        return lib.tms_page_tables(lengths, n, nul, 2, nul, p, 4, page, po, p, ids, p, cap, nul, 0, ws, wsb, nul)
+    def tables(lengths=p, n=5000, page=32, po=p, ids=p, cap=4, ws=p, wsb=1 << 20):
+        return lib.tms_page_tables(lengths, n, nul, 5000, nul, p, 4, page, po, p, ids, p, cap, nul, 0, ws, wsb, nul)
 
     assert tables(page=24) == L.TMS_ERR_UNSUPPORTED
     assert tables(n=1) == L.TMS_ERR_INVALID  # fewer lengths than documents

@@ -6,6 +6,7 @@ entry point raises -- there is no CPU or eager fallback. Buffers are passed as r
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -62,7 +63,7 @@ SIGNATURES = {
     "tms_residual_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
     "tms_residual_maxsim": (_i32, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i64, _vp, _i64,
                                    _i64, _vp, _vp, _sz, _vp]),
-    "tms_page_tables_workspace_size": (_sz, [_i64]),
+    "tms_page_tables_workspace_size": (_sz, [_i64, _i64]),
     "tms_page_tables": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64,
                                _vp, _sz, _vp]),
     "tms_page_write": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _i32, ctypes.c_float, _i64, _i64, _vp,
@@ -115,7 +116,13 @@ def check(code: int, what: str) -> None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(index)  # torch.cuda.current_stream(device).cuda_stream, without the object
+
+
+def on_device(device: torch.device):
+    """torch.cuda.device(device), or nothing where that device is current already."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def require_cuda(*tensors: torch.Tensor) -> torch.device:

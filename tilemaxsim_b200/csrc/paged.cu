@@ -39,11 +39,13 @@ struct TableArgs {
   int64_t page_cap;
   int64_t* slots;          // (token_cap,) or nullptr
   int64_t token_cap;
-  int64_t* tile_sums;      // workspace: (tiles, 2) pages and tokens of each tile of documents
+  int64_t* tile_sums;      // workspace: (tiles, 2) pages and tokens of each tile of documents,
+  int32_t* owners;         // and the document that owns each 32nd table entry
 };
 
 constexpr int kTableThreads = 256;
 constexpr int kTileDocs = 1024;  // documents of one tile (four for each thread)
+constexpr int kFewDocs = 2048;   // documents whose offsets a CTA works out for itself
 
 // Document i's length; an id outside the store has none, a negative length counts as zero, and one
 // of 2^31 or more, which no pool holds, as 2^31 - 1 (so that no sum of lengths overflows).
@@ -132,6 +134,9 @@ __global__ void __launch_bounds__(kTableThreads) table_offsets_kernel(const Tabl
     if (i < a.n_docs) {
       a.page_offsets[i] = bp + p;
       a.token_offsets[i] = bt + t;
+      // the entries 32 b of this document
+      const int64_t end = bp + p + ((len + round) >> a.page_shift), most = a.page_cap;
+      for (int64_t b = (bp + p + 31) >> 5; (b << 5) < (end < most ? end : most); ++b) a.owners[b] = static_cast<int32_t>(i);
     }
     bp += tp;
     bt += tt;
@@ -142,9 +147,8 @@ __global__ void __launch_bounds__(kTableThreads) table_offsets_kernel(const Tabl
   }
 }
 
-// The last document d in [0, n_docs) with page_offsets[d] <= k (k lies below the total).
-__device__ __forceinline__ int64_t owner_of(const int64_t* page_offsets, int64_t n_docs, int64_t k) {
-  int64_t lo = 0, hi = n_docs;  // the first offset above k is in (lo, hi]
+// The last document d in [lo, hi) with page_offsets[d] <= k, which page_offsets[lo] is.
+__device__ __forceinline__ int64_t owner_of(const int64_t* page_offsets, int64_t lo, int64_t hi, int64_t k) {
   while (hi - lo > 1) {
     const int64_t mid = (lo + hi) >> 1;
     if (page_offsets[mid] <= k) lo = mid;
@@ -153,48 +157,150 @@ __device__ __forceinline__ int64_t owner_of(const int64_t* page_offsets, int64_t
   return lo;
 }
 
-// Page ids, owners and token slots: a warp takes 32 consecutive table entries, finds their owners
-// (a lane for each) and then writes the slots of one page after the other.
+// Page ids, owners and slots of the 32 table entries from k0 on, by one warp: a lane for each entry
+// (`doc` owns it, where it lies below the total), then the entries' slots one after the other. The
+// entries' tokens follow one another, so one base and 32-bit distances from it place them.
+__device__ __forceinline__ void fill_entries(const TableArgs& a, int64_t k0, int64_t total, int64_t doc,
+                                             int64_t doc_page, int64_t doc_token, int64_t doc_end) {
+  constexpr uint32_t kAllWarp = 0xffffffffu;
+  const int lane = threadIdx.x & 31;
+  const int page = 1 << a.page_shift;
+  const int64_t k = k0 + lane;
+  const bool used = k < total && k < a.page_cap;
+  int64_t tok = 0;
+  int id = -1, count = 0;
+  if (used) {
+    const int64_t nth = k - doc_page;
+    int64_t src = k;
+    if (a.src_offsets) src = __ldg(a.src_offsets + (a.doc_ids ? __ldg(a.doc_ids + doc) : doc)) + nth;
+    if (src >= 0 && src < a.n_src) id = __ldg(a.pages + src);
+    tok = doc_token + (nth << a.page_shift);
+    count = static_cast<int>(doc_end - tok < page ? doc_end - tok : page);
+  }
+  if (k < a.page_cap) {
+    a.page_ids[k] = id;
+    a.page_docs[k] = used ? static_cast<int32_t>(doc) : -1;
+  }
+  if (!a.slots) return;
+  const int64_t base = __shfl_sync(kAllWarp, tok, 0);
+  const int at = static_cast<int>(tok - base);
+  int64_t* const to = a.slots + base;
+  const int64_t room = a.token_cap - base;
+  const int entries = __popc(__ballot_sync(kAllWarp, used));
+  const int last_at = __shfl_sync(kAllWarp, at + count, entries > 0 ? entries - 1 : 0);
+  const bool fits = last_at <= room;
+#pragma unroll 4
+  for (int l = 0; l < entries; ++l) {
+    const int n = __shfl_sync(kAllWarp, count, l), t = __shfl_sync(kAllWarp, at, l), p = __shfl_sync(kAllWarp, id, l);
+    const int64_t first = p < 0 ? -1 : static_cast<int64_t>(p) << a.page_shift;
+    for (int j = lane; j < n; j += 32)
+      if (fits || t + j < room) to[t + j] = p < 0 ? -1 : first + j;
+  }
+}
+
+// Slots that no entry covers, from token `rest` on.
+__device__ __forceinline__ void fill_rest(const TableArgs& a, int64_t rest) {
+  if (!a.slots) return;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t t = rest + static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; t < a.token_cap; t += step)
+    a.slots[t] = -1;
+}
+
+// A warp takes 32 consecutive table entries at a time. Its first entry's owner is in the workspace,
+// the others' are among the next documents, whose offsets a lane each loads at once.
 __global__ void __launch_bounds__(kTableThreads) table_fill_kernel(const TableArgs a) {
+  constexpr uint32_t kAllWarp = 0xffffffffu;
   const int lane = threadIdx.x & 31;
   const int64_t warps = static_cast<int64_t>(gridDim.x) * (kTableThreads / 32);
   const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kTableThreads / 32) + (threadIdx.x >> 5);
   const int64_t total = a.page_offsets[a.n_docs];
-  const int64_t page = int64_t(1) << a.page_shift;
   for (int64_t k0 = warp * 32; k0 < a.page_cap; k0 += warps * 32) {
     const int64_t k = k0 + lane;
-    int64_t tok = 0, id = -1, doc = -1;
-    int count = 0;
-    if (k < total && k < a.page_cap) {
-      doc = owner_of(a.page_offsets, a.n_docs, k);
-      const int64_t nth = k - a.page_offsets[doc];
-      const int64_t t0 = a.token_offsets[doc], t1 = a.token_offsets[doc + 1];
-      int64_t src = k;
-      if (a.src_offsets) src = __ldg(a.src_offsets + (a.doc_ids ? __ldg(a.doc_ids + doc) : doc)) + nth;
-      if (src >= 0 && src < a.n_src) id = __ldg(a.pages + src);
-      tok = t0 + nth * page;
-      count = static_cast<int>(t1 - tok < page ? t1 - tok : page);
+    int64_t doc = 0, doc_page = 0, doc_token = 0, doc_end = 0;
+    if (k0 < total) {
+      const int64_t lo = a.owners[k0 >> 5];
+      const int64_t next = lo + 1 + lane;
+      const int64_t starts = a.page_offsets[next < a.n_docs ? next : a.n_docs];  // where document `next` starts
+      int d = 0;  // documents after lo that start at or before k
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1)
+        if (__shfl_sync(kAllWarp, starts, d + w - 1) <= k) d += w;
+      const int64_t last = __shfl_sync(kAllWarp, starts, 31);  // all lanes take part, before any is left out
+      const bool beyond = d == 31 && last <= k;
+      doc = lo + d;
+      if (beyond && k < total) doc = owner_of(a.page_offsets, lo, a.n_docs, k);  // many empty documents
+      if (k < total) {
+        doc_page = a.page_offsets[doc];
+        doc_token = a.token_offsets[doc];
+        doc_end = a.token_offsets[doc + 1];
+      }
     }
-    if (k < a.page_cap) {
-      a.page_ids[k] = static_cast<int32_t>(id);
-      a.page_docs[k] = static_cast<int32_t>(doc);
-    }
-    if (!a.slots) continue;
-    for (int l = 0; l < 32; ++l) {
-      const int n = __shfl_sync(0xffffffffu, count, l);
-      const int64_t t = __shfl_sync(0xffffffffu, tok, l);
-      const int64_t pid = __shfl_sync(0xffffffffu, id, l);
-      for (int j = lane; j < n; j += 32)
-        if (t + j < a.token_cap) a.slots[t + j] = pid < 0 ? -1 : (pid << a.page_shift) + j;
-    }
+    fill_entries(a, k0, total, doc, doc_page, doc_token, doc_end);
   }
-  if (!a.slots) return;
   int64_t rest = a.token_offsets[a.n_docs];  // tokens from here on have no table entry
   if (total > a.page_cap) {
-    const int64_t doc = owner_of(a.page_offsets, a.n_docs, a.page_cap);
+    const int64_t doc = owner_of(a.page_offsets, 0, a.n_docs, a.page_cap);
     rest = a.token_offsets[doc] + ((a.page_cap - a.page_offsets[doc]) << a.page_shift);
   }
-  for (int64_t t = rest + warp * 32 + lane; t < a.token_cap; t += warps * 32) a.slots[t] = -1;
+  fill_rest(a, rest);
+}
+
+// Few documents, in one launch: every CTA works out all offsets in shared memory (eight documents
+// a thread) and fills its part of the tables; the first one also writes the offsets.
+__global__ void __launch_bounds__(kTableThreads) table_few_kernel(const TableArgs a) {
+  __shared__ int64_t pages[kFewDocs + 1], tokens[kFewDocs + 1];
+  __shared__ int64_t sh[kTableThreads / 32][2];
+  constexpr int kEach = kFewDocs / kTableThreads;
+  const int lane = threadIdx.x & 31;
+  const int n = static_cast<int>(a.n_docs);
+  const int64_t round = (int64_t(1) << a.page_shift) - 1;
+  const int each = (n + kTableThreads - 1) / kTableThreads;  // documents of a thread
+  const int i0 = threadIdx.x * each;
+  int64_t len[kEach], p = 0, t = 0, total, total_tokens;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    len[j] = j < each && i0 + j < n ? table_length(a, i0 + j) : 0;
+    p += (len[j] + round) >> a.page_shift;
+    t += len[j];
+  }
+  block_scan2(p, t, &total, &total_tokens, sh);
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    if (j >= each || i0 + j >= n) break;
+    pages[i0 + j] = p;
+    tokens[i0 + j] = t;
+    p += (len[j] + round) >> a.page_shift;
+    t += len[j];
+  }
+  if (threadIdx.x == 0) {
+    pages[n] = total;
+    tokens[n] = total_tokens;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i <= n; i += kTableThreads) {
+      a.page_offsets[i] = pages[i];
+      a.token_offsets[i] = tokens[i];
+    }
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kTableThreads / 32);
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kTableThreads / 32) + (threadIdx.x >> 5);
+  for (int64_t k0 = warp * 32; k0 < a.page_cap; k0 += warps * 32) {
+    const int64_t k = k0 + lane;
+    int64_t doc = 0, doc_page = 0, doc_token = 0, doc_end = 0;
+    if (k < total) {
+      doc = owner_of(pages, 0, n, k);
+      doc_page = pages[doc];
+      doc_token = tokens[doc];
+      doc_end = tokens[doc + 1];
+    }
+    fill_entries(a, k0, total, doc, doc_page, doc_token, doc_end);
+  }
+  int64_t rest = total_tokens;
+  if (total > a.page_cap) {
+    const int64_t doc = owner_of(pages, 0, n, a.page_cap);
+    rest = tokens[doc] + ((a.page_cap - pages[doc]) << a.page_shift);
+  }
+  fill_rest(a, rest);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -740,9 +846,10 @@ bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) 
 
 using namespace tms;
 
-extern "C" size_t tms_page_tables_workspace_size(int64_t n_docs) {
-  if (n_docs <= 0) return 0;
-  return static_cast<size_t>((n_docs + kTileDocs - 1) / kTileDocs) * 16;
+extern "C" size_t tms_page_tables_workspace_size(int64_t n_docs, int64_t page_capacity) {
+  if (n_docs <= kFewDocs || page_capacity < 0) return 0;
+  return static_cast<size_t>((n_docs + kTileDocs - 1) / kTileDocs) * 16 +
+         align_up(static_cast<size_t>(page_capacity / 32 + 1) * 4, 16);
 }
 
 extern "C" int tms_page_tables(const int64_t* lengths, int64_t n_lengths, const int64_t* doc_ids,
@@ -761,23 +868,29 @@ extern "C" int tms_page_tables(const int64_t* lengths, int64_t n_lengths, const 
   if (!page_offsets || !token_offsets || (n_lengths > 0 && !lengths) || (n_src_pages > 0 && !pages) ||
       (page_capacity > 0 && (!page_ids || !page_docs)))
     return TMS_ERR_INVALID;
-  if (n_docs > 0 && (!workspace || workspace_bytes < tms_page_tables_workspace_size(n_docs)))
-    return TMS_ERR_WORKSPACE;
+  const size_t need = tms_page_tables_workspace_size(n_docs, page_capacity);
+  if (need && (!workspace || workspace_bytes < need)) return TMS_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 7) return TMS_ERR_INVALID;
   int status = TMS_OK;
   const DeviceInfo* dev = current_device_info(&status);
   if (!dev) return status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t tiles = (n_docs + kTileDocs - 1) / kTileDocs;
+  int64_t* const sums = static_cast<int64_t*>(workspace);
   const TableArgs a{lengths, n_lengths, doc_ids, n_docs, src_offsets, pages, n_src_pages, shift, page_offsets,
                     token_offsets, page_ids, page_docs, page_capacity, slots, slots ? token_capacity : 0,
-                    static_cast<int64_t*>(workspace)};
-  const int64_t tiles = n_docs > 0 ? (n_docs + kTileDocs - 1) / kTileDocs : 1;
-  if (tiles > 1) table_sums_kernel<<<static_cast<unsigned>(tiles), kTableThreads, 0, st>>>(a);
-  table_offsets_kernel<<<static_cast<unsigned>(tiles), kTableThreads, 0, st>>>(a);
+                    sums, reinterpret_cast<int32_t*>(sums + 2 * tiles)};
   int64_t blocks = (page_capacity + kTableThreads - 1) / kTableThreads;
   const int64_t most = static_cast<int64_t>(dev->num_sms) * 8;
   blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
-  table_fill_kernel<<<static_cast<unsigned>(blocks), kTableThreads, 0, st>>>(a);
+  if (n_docs <= kFewDocs) {
+    if (blocks > dev->num_sms) blocks = dev->num_sms;  // each CTA works out the offsets
+    table_few_kernel<<<static_cast<unsigned>(blocks), kTableThreads, 0, st>>>(a);
+  } else {
+    table_sums_kernel<<<static_cast<unsigned>(tiles), kTableThreads, 0, st>>>(a);
+    table_offsets_kernel<<<static_cast<unsigned>(tiles), kTableThreads, 0, st>>>(a);
+    table_fill_kernel<<<static_cast<unsigned>(blocks), kTableThreads, 0, st>>>(a);
+  }
   return cuda_status(cudaGetLastError());
 }
 

@@ -15,7 +15,6 @@ The reference has no such corpus: its corpora are fixed tensors (src/flash_maxsi
 """
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple
 
 import torch
@@ -40,8 +39,8 @@ class PageTables(NamedTuple):
     slots: torch.Tensor | None
 
 
-def _ptr(t: torch.Tensor | None) -> ctypes.c_void_p:
-    return ctypes.c_void_p(t.data_ptr() if t is not None else 0)
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def _page_size(page_size: int) -> int:
@@ -51,9 +50,9 @@ def _page_size(page_size: int) -> int:
 
 
 def _ints(t: torch.Tensor, dtype: torch.dtype, name: str) -> torch.Tensor:
-    if t.dim() != 1 or t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+    if t.dim() != 1 or (t.dtype != dtype and (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool)):
         raise ValueError(f"{name} must be a 1-D integer tensor, got {t.dtype} {tuple(t.shape)}")
-    return t.to(dtype).contiguous()
+    return (t if t.dtype == dtype else t.to(dtype)).contiguous()
 
 
 def _tables_call(lengths, doc_ids, src_offsets, pages, page_size, n_tokens, with_slots) -> PageTables:
@@ -62,18 +61,18 @@ def _tables_call(lengths, doc_ids, src_offsets, pages, page_size, n_tokens, with
     dev = _lib.require_cuda(*given)
     n_docs = lengths.numel() if doc_ids is None else doc_ids.numel()
     capacity = (n_tokens + n_docs * (page_size - 1)) // page_size
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         def empty(n, dtype):
             return torch.empty(n, dtype=dtype, device=dev)
         out = PageTables(empty(n_docs + 1, torch.int64), empty(capacity, torch.int32), empty(capacity, torch.int32),
                          empty(n_docs + 1, torch.int64), empty(n_tokens, torch.int64) if with_slots else None)
-        ws_bytes = lib.tms_page_tables_workspace_size(n_docs)
+        ws_bytes = lib.tms_page_tables_workspace_size(n_docs, capacity)
         ws, ws_ptr = _lib.workspace(ws_bytes, dev, align=256)
         rc = lib.tms_page_tables(
             _ptr(lengths), lengths.numel(), _ptr(doc_ids), n_docs, _ptr(src_offsets), _ptr(pages), pages.numel(),
             page_size, _ptr(out.page_offsets), _ptr(out.token_offsets), _ptr(out.page_ids), _ptr(out.page_docs),
-            capacity, _ptr(out.slots), n_tokens, ctypes.c_void_p(ws_ptr), ws_bytes,
-            ctypes.c_void_p(_lib.stream_handle(dev)))
+            capacity, _ptr(out.slots), n_tokens, ws_ptr, ws_bytes,
+            _lib.stream_handle(dev))
         _lib.check(rc, "tms_page_tables")
         del ws
     return out
@@ -177,7 +176,7 @@ def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales:
     def fits(t):
         return t.stride(-1) == 1 and all(s % rows == 0 and s >= 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
 
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         if not fits(x) or (residual is not None and (not fits(residual) or residual.stride() != x.stride())):
             x = x.clone(memory_format=torch.contiguous_format)
             residual = None if residual is None else residual.clone(memory_format=torch.contiguous_format)
@@ -188,7 +187,7 @@ def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales:
             _ptr(x), _lib.DTYPE_CODE[x.dtype], x.shape[-2], x.stride(0) if padded else 0, x.stride(-2), int(padded),
             _ptr(residual), _ptr(weight), _NORMS[norm], eps, d, page_size, _ptr(tables.page_offsets),
             _ptr(tables.token_offsets), _ptr(tables.page_ids), _ptr(tables.page_docs), n_docs,
-            tables.page_ids.numel(), _ptr(codes), _ptr(scales), n_pages, ctypes.c_void_p(_lib.stream_handle(dev)))
+            tables.page_ids.numel(), _ptr(codes), _ptr(scales), n_pages, _lib.stream_handle(dev))
         _lib.check(rc, "tms_page_write")
     return codes, scales
 
@@ -203,10 +202,10 @@ def page_read(codes: torch.Tensor, scales: torch.Tensor, slots: torch.Tensor,
         raise TypeError(f"unsupported dtype {dtype}; use float16, bfloat16 or float32")
     slots = _ints(slots, torch.int64, "slots")
     dev = _lib.require_cuda(codes, scales, slots)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         out = torch.empty((slots.numel(), d), dtype=dtype, device=dev)
         rc = lib.tms_page_read(_ptr(codes), _ptr(scales), n_pages, page_size, d, _ptr(slots), slots.numel(),
-                               _ptr(out), _lib.DTYPE_CODE[dtype], ctypes.c_void_p(_lib.stream_handle(dev)))
+                               _ptr(out), _lib.DTYPE_CODE[dtype], _lib.stream_handle(dev))
         _lib.check(rc, "tms_page_read")
     return out
 
@@ -233,7 +232,7 @@ def paged_maxsim(Qb: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, ta
     Bq, Nq, _ = Qb.shape
     if Nq == 0:
         raise ValueError("a query needs at least one token")
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         Qb = Qb.contiguous()
         Qb = Qb if Qb.data_ptr() % 16 == 0 else Qb.clone()
         out = torch.empty((Bq, n_docs), dtype=torch.float32, device=dev)
@@ -243,8 +242,8 @@ def paged_maxsim(Qb: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, ta
             rc = lib.tms_paged_maxsim(
                 _ptr(Qb), _lib.DTYPE_CODE[Qb.dtype], Bq, Nq, d, _ptr(codes), _ptr(scales), n_pages, page_size,
                 _ptr(tables.page_offsets), _ptr(tables.page_ids), _ptr(tables.page_docs), n_docs,
-                tables.page_ids.numel(), _ptr(out), ctypes.c_void_p(ws_ptr), ws_bytes,
-                ctypes.c_void_p(_lib.stream_handle(dev)))
+                tables.page_ids.numel(), _ptr(out), ws_ptr, ws_bytes,
+                _lib.stream_handle(dev))
             _lib.check(rc, "tms_paged_maxsim")
             del ws
     return out[0] if single else out
