@@ -189,12 +189,23 @@ __device__ __forceinline__ void fill_entries(const TableArgs& a, int64_t k0, int
   const int entries = __popc(__ballot_sync(kAllWarp, used));
   const int last_at = __shfl_sync(kAllWarp, at + count, entries > 0 ? entries - 1 : 0);
   const bool fits = last_at <= room;
-#pragma unroll 4
+  const int place = at << 8 | count;  // at most 4,064 and 128
+  if (fits && !__any_sync(kAllWarp, used && id < 0)) {
+    // every slot is there: 32 of them an instruction, of one page or of two
+    const int each = page < 32 ? 32 >> a.page_shift : 1, j = page < 32 ? lane & (page - 1) : lane;
+    const int sub = page < 32 ? lane >> a.page_shift : 0;
+    for (int from = 0; from < page; from += page < 32 ? page : 32)
+#pragma unroll 8
+      for (int l = 0; l < 32; l += each) {
+        const int w = __shfl_sync(kAllWarp, place, l + sub), p = __shfl_sync(kAllWarp, id, l + sub);
+        if (from + j < (w & 0xff)) to[(w >> 8) + from + j] = (static_cast<int64_t>(p) << a.page_shift) + from + j;
+      }
+    return;
+  }
   for (int l = 0; l < entries; ++l) {
-    const int n = __shfl_sync(kAllWarp, count, l), t = __shfl_sync(kAllWarp, at, l), p = __shfl_sync(kAllWarp, id, l);
-    const int64_t first = p < 0 ? -1 : static_cast<int64_t>(p) << a.page_shift;
-    for (int j = lane; j < n; j += 32)
-      if (fits || t + j < room) to[t + j] = p < 0 ? -1 : first + j;
+    const int w = __shfl_sync(kAllWarp, place, l), p = __shfl_sync(kAllWarp, id, l);
+    for (int j = lane; j < (w & 0xff); j += 32)
+      if ((w >> 8) + j < room) to[(w >> 8) + j] = p < 0 ? -1 : (static_cast<int64_t>(p) << a.page_shift) + j;
   }
 }
 
@@ -801,35 +812,77 @@ struct ReadArgs {
   void* out;
 };
 
-// out[t] = scale * code of slot t; a slot outside the pool gives a row of zeros. A thread takes
-// eight elements. One multiplication in fp32, then one rounding to the output type.
+// out[t] = scale * code of slot t; a slot outside the pool gives a row of zeros. One multiplication
+// in fp32, then one rounding to the output type. A group of lanes takes a row, sixteen elements a
+// lane (one 16-byte load), and a thread four rows, whose loads are all in flight before the first
+// store: what bounds it is memory. The output is written past the caches' working set.
+constexpr int kReadRows = 4;
+
 template <typename T>
-__global__ void page_read_kernel(const ReadArgs a) {
-  const int vecs = a.d >> 3;
-  const int64_t n = a.n_slots * vecs;
-  for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < n;
-       e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t t = e / vecs;
-    const int sub = static_cast<int>(e - t * vecs);
-    const int64_t slot = a.slots[t];
-    alignas(16) T v[8];
-    if (slot >= 0 && (slot >> a.page_shift) < a.n_pages) {
-      const uint2 c = *reinterpret_cast<const uint2*>(a.codes + slot * a.d + sub * 8);
-      const float s = a.scales[slot >> a.page_shift];
-      const uint8_t* b = reinterpret_cast<const uint8_t*>(&c);
+__device__ __forceinline__ uint32_t two_as(float x, float y) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ float2 e4m3x2_value(uint32_t two) {
+  uint32_t h;
+  asm("{\n\t.reg .b16 p;\n\tcvt.u16.u32 p, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, p;\n\t}\n" : "=r"(h) : "r"(two));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) page_read_kernel(const ReadArgs a, int group) {
+  const int sub = threadIdx.x & (group - 1);
+  const int64_t rows = 256 / group;  // of a CTA at a time
+  const bool in_row = sub * 16 < a.d;
+  for (int64_t t0 = blockIdx.x * rows * kReadRows + threadIdx.x / group; t0 < a.n_slots;
+       t0 += gridDim.x * rows * kReadRows) {
+    int64_t slot[kReadRows];
+    uint4 c[kReadRows];
+    float scale[kReadRows];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const __half_raw h = __nv_cvt_fp8_to_halfraw(b[i], __NV_E4M3);
-        v[i] = static_cast<T>(__half2float(__half(h)) * s);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(0.f);
+    for (int i = 0; i < kReadRows; ++i) {
+      const int64_t t = t0 + i * rows;
+      slot[i] = t < a.n_slots ? __ldg(a.slots + t) : -1;
     }
-    T* const o = static_cast<T*>(a.out) + t * a.d + sub * 8;
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-      reinterpret_cast<uint4*>(o)[i] = reinterpret_cast<const uint4*>(v)[i];
+    for (int i = 0; i < kReadRows; ++i) {
+      c[i] = make_uint4(0, 0, 0, 0);
+      scale[i] = 0.f;
+      if (slot[i] >= 0 && (slot[i] >> a.page_shift) < a.n_pages && in_row) {
+        c[i] = __ldg(reinterpret_cast<const uint4*>(a.codes + slot[i] * a.d + sub * 16));
+        scale[i] = __ldg(a.scales + (slot[i] >> a.page_shift));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kReadRows; ++i) {
+      const int64_t t = t0 + i * rows;
+      if (t >= a.n_slots || !in_row) continue;
+      const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 f = e4m3x2_value(w[j >> 1] >> (16 * (j & 1)) & 0xffffu);
+        v[2 * j] = f.x * scale[i];
+        v[2 * j + 1] = f.y * scale[i];
+      }
+      uint4* const o = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + t * a.d + sub * 16);
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          __stcs(o + q, make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]),
+                                   __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3])));
+      } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          __stcs(o + q, make_uint4(two_as<T>(v[8 * q], v[8 * q + 1]), two_as<T>(v[8 * q + 2], v[8 * q + 3]),
+                                   two_as<T>(v[8 * q + 4], v[8 * q + 5]), two_as<T>(v[8 * q + 6], v[8 * q + 7])));
+      }
+    }
   }
 }
 
@@ -944,12 +997,16 @@ extern "C" int tms_page_read(const void* codes, const float* scales, int64_t n_p
   if (!dev) return status;
   const ReadArgs a{static_cast<const uint8_t*>(codes), scales, n_pages, shift, static_cast<int>(d), slots,
                    n_slots, out};
-  int64_t blocks = (n_slots * (d / 8) + 255) / 256;
+  int group = 1;  // lanes of a row
+  while (group * 16 < d) group <<= 1;
+  const int64_t rows = 256 / group * kReadRows;
+  int64_t blocks = (n_slots + rows - 1) / rows;
   const int64_t most = static_cast<int64_t>(dev->num_sms) * 16;
   if (blocks > most) blocks = most;
+  const unsigned grid = static_cast<unsigned>(blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (out_dtype == TMS_F16) page_read_kernel<__half><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
-  else if (out_dtype == TMS_BF16) page_read_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
-  else page_read_kernel<float><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+  if (out_dtype == TMS_F16) page_read_kernel<__half><<<grid, 256, 0, st>>>(a, group);
+  else if (out_dtype == TMS_BF16) page_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, group);
+  else page_read_kernel<float><<<grid, 256, 0, st>>>(a, group);
   return cuda_status(cudaGetLastError());
 }

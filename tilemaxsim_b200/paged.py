@@ -43,6 +43,14 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _device(*tensors: torch.Tensor) -> torch.device:
+    """The tensors' common CUDA device (as _lib.require_cuda, which says what is wrong where it is not)."""
+    index = tensors[0].get_device()
+    if index < 0 or any([t.get_device() != index for t in tensors]):
+        return _lib.require_cuda(*tensors)
+    return tensors[0].device
+
+
 def _page_size(page_size: int) -> int:
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
@@ -58,7 +66,7 @@ def _ints(t: torch.Tensor, dtype: torch.dtype, name: str) -> torch.Tensor:
 def _tables_call(lengths, doc_ids, src_offsets, pages, page_size, n_tokens, with_slots) -> PageTables:
     lib = _lib.load()
     given = [t for t in (lengths, doc_ids, src_offsets, pages) if t is not None]
-    dev = _lib.require_cuda(*given)
+    dev = _device(*given)
     n_docs = lengths.numel() if doc_ids is None else doc_ids.numel()
     capacity = (n_tokens + n_docs * (page_size - 1)) // page_size
     with _lib.on_device(dev):
@@ -158,7 +166,7 @@ def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales:
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     n_pages, page_size, d = _check_pool(codes, scales)
     n_docs = _check_tables(tables)
-    dev = _lib.require_cuda(x, codes, scales, tables.page_offsets, tables.page_ids, tables.page_docs,
+    dev = _device(x, codes, scales, tables.page_offsets, tables.page_ids, tables.page_docs,
                             tables.token_offsets, *(t for t in (residual, weight) if t is not None))
     if x.dtype not in _lib.DTYPE_CODE:
         raise TypeError(f"unsupported dtype {x.dtype}; use float16, bfloat16 or float32")
@@ -201,7 +209,7 @@ def page_read(codes: torch.Tensor, scales: torch.Tensor, slots: torch.Tensor,
     if dtype not in _lib.DTYPE_CODE:
         raise TypeError(f"unsupported dtype {dtype}; use float16, bfloat16 or float32")
     slots = _ints(slots, torch.int64, "slots")
-    dev = _lib.require_cuda(codes, scales, slots)
+    dev = _device(codes, scales, slots)
     with _lib.on_device(dev):
         out = torch.empty((slots.numel(), d), dtype=dtype, device=dev)
         rc = lib.tms_page_read(_ptr(codes), _ptr(scales), n_pages, page_size, d, _ptr(slots), slots.numel(),
@@ -222,7 +230,7 @@ def paged_maxsim(Qb: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, ta
     single = Qb.dim() == 2
     if single:
         Qb = Qb.unsqueeze(0)
-    dev = _lib.require_cuda(Qb, codes, scales, tables.page_offsets, tables.page_ids, tables.page_docs)
+    dev = _device(Qb, codes, scales, tables.page_offsets, tables.page_ids, tables.page_docs)
     if Qb.dim() != 3 or Qb.shape[2] != d:
         raise ValueError(f"expected Q (B_q, Nq, {d}) or (Nq, {d}), got {tuple(Qb.shape)}")
     if Qb.dtype == torch.float32:
