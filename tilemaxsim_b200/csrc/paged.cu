@@ -399,7 +399,7 @@ struct Eight {
   }
 };
 
-// One page at a time a CTA of four warps, the next page on its way into shared memory (cp.async)
+// One page at a time a CTA of two or four warps, the next page on its way into shared memory (cp.async)
 // meanwhile; a group of 2 to 32 lanes takes a row, eight elements a lane. The input is read from
 // memory once and the codes are written once, which bounds the kernel. Pages of more than
 // kStageBytes of input are read twice instead, the second time from the caches.
@@ -417,10 +417,11 @@ struct Eight {
 __device__ __forceinline__ double max_keep_nan(double x, double y) { return y <= x || x != x ? x : y; }
 __device__ __forceinline__ bool usual(float v) { return v >= 1e-30f && v <= 1e30f; }
 
-#ifndef WT
-#define WT 64
-#endif
-constexpr int kWriteThreads = WT;
+// Threads of a CTA: 64 where a page's input is 16-bit values alone; 128 where twice the input leaves
+// room for half as many CTAs (1,024 documents with a residual: 72 us with 64, 61 with 128), and
+// where pages are not staged.
+template <typename T, bool SUM, bool STAGED>
+constexpr int write_threads() { return sizeof(T) == 2 && !SUM && STAGED ? 64 : 128; }
 constexpr int kStageBytes = 24 * 1024;  // most input of a page (x and residual) that is staged
 
 struct Entry {    // where a table entry's rows come from
@@ -512,7 +513,9 @@ __device__ __forceinline__ void exact_row(const PageRows<T, SUM, WEIGHT, STAGED>
 }
 
 template <typename T, bool SUM, bool WEIGHT, bool STAGED>
-__global__ void __launch_bounds__(kWriteThreads, 1024 / kWriteThreads) page_write_kernel(const WriteArgs a, int group) {
+__global__ void __launch_bounds__(write_threads<T, SUM, STAGED>(), 1024 / write_threads<T, SUM, STAGED>())
+page_write_kernel(const WriteArgs a, int group) {
+  constexpr int kWriteThreads = write_threads<T, SUM, STAGED>();
   constexpr uint32_t kAllWarp = 0xffffffffu;
   constexpr int kWarps = kWriteThreads / 32;
   extern __shared__ __align__(16) uint8_t stage_bytes[];
@@ -780,15 +783,17 @@ cudaError_t launch_write_as(const WriteArgs& a, const DeviceInfo* dev, cudaStrea
   while (group * 8 < a.d) group <<= 1;
   const int input = (a.d << a.page_shift) * static_cast<int>(sizeof(T)) * (SUM ? 2 : 1);
   const bool staged = input <= kStageBytes;
-  const int64_t most = static_cast<int64_t>(dev->num_sms) * 12;
+  // As many CTAs as fit at a time: each then has its next page on the way while it works on one.
+  const int fit = staged ? dev->max_smem_optin / (2 * input + 2048) : 16;
+  const int64_t most = static_cast<int64_t>(dev->num_sms) * (fit < 16 ? fit : 16);
   const unsigned blocks = static_cast<unsigned>(a.page_cap < most ? a.page_cap : most);
   if (staged) {
     auto kern = page_write_kernel<T, SUM, WEIGHT, true>;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStageBytes);
     if (e != cudaSuccess) return e;
-    kern<<<blocks, kWriteThreads, 2 * input, st>>>(a, group);
+    kern<<<blocks, write_threads<T, SUM, true>(), 2 * input, st>>>(a, group);
   } else {
-    page_write_kernel<T, SUM, WEIGHT, false><<<blocks, kWriteThreads, 0, st>>>(a, group);
+    page_write_kernel<T, SUM, WEIGHT, false><<<blocks, write_threads<T, SUM, false>(), 0, st>>>(a, group);
   }
   return cudaGetLastError();
 }

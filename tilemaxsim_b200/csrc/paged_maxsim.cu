@@ -185,6 +185,9 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
                : "memory");
 }
+// The packed queries come from the launch before this one, which this one does not wait to end.
+__device__ __forceinline__ void wait_for_packed() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // A value that is the same in all lanes, told to the compiler.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
@@ -287,8 +290,10 @@ __device__ __forceinline__ void pack_rows(const PagedArgs& a, int nc, int m, int
   }
 }
 
-// All M tiles (of four chunks) of a call, for CTAs that hold several: packed once, not by each CTA.
+// All M tiles (of four chunks) of a call, packed once, not by each CTA: 128 rows took a CTA 7 us. The
+// scoring kernel's CTAs start meanwhile and find their streams.
 __global__ void __launch_bounds__(256) paged_pack_kernel(const PagedArgs a, uint8_t* packed, float* factor) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t row = (static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * kPackRows;
   const int m = static_cast<int>(row >> 7);
   if (m < a.n_mtiles)
@@ -348,8 +353,9 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       fence_mbar_init();
     }
     const int64_t total = clamp_entry(a, __ldg(a.page_offsets + a.n_docs));
-    const int64_t lo = cut_at(a, total, range, a.ranges);
-    int64_t hi = cut_at(a, total, range + 1, a.ranges);
+    const int64_t cut = lane < 2 ? cut_at(a, total, range + lane, a.ranges) : 0;
+    const int64_t lo = __shfl_sync(kAllWarp, cut, 0);
+    int64_t hi = __shfl_sync(kAllWarp, cut, 1);
     hi = hi < lo ? lo : hi;
     const int64_t first = lo + (hi - lo) * lane / kStreams;  // of stream `lane`
     const int64_t next = lo + (hi - lo) * (lane + 1) / kStreams;
@@ -370,6 +376,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
     asm volatile("barrier.arrive %0, %1;" ::"r"(kReadyBarrier), "r"(kThreads) : "memory");
     if (a.packed && !dead && n_tiles > 0) {
       if (lane == 0) {
+        wait_for_packed();
         mbar_arrive_expect_tx(query_bar, static_cast<uint32_t>(mt) * L.q_bytes);
         for (int m = 0; m < mt; ++m)
           bulk_load(base + L.q + static_cast<uint32_t>(m) * L.q_bytes,
@@ -384,9 +391,9 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
     }
     float* const factor = reinterpret_cast<float*>(smem + L.factor);
     if (a.packed) {
-      for (int i = threadIdx.x - 32; i < mt * 128; i += kThreads - 32)
-        factor[i] = __ldg(a.packed_factor + m_first * 128 + i);
-    } else {  // one M tile
+      wait_for_packed();
+      for (int i = threadIdx.x - 32; i < mt * 128; i += kThreads - 32) factor[i] = a.packed_factor[m_first * 128 + i];
+    } else {  // one or two chunks
       for (int r0 = (warp - 1) * kPackRows; r0 < 32 * NC; r0 += 9 * kPackRows)
         pack_rows(a, NC, m_first, r0, smem + L.q, factor);
       fence_proxy_async_smem();  // the tensor core reads what the packing wrote
@@ -551,6 +558,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       float cur_scale = 0.f, next_scale = 0.f;
       int cur_ends = -1, next_ends = -1;
       uint32_t end_mask = 0;  // a bit for each of the 32 boxes with which a document ends
+      uint32_t odd_mask = 0;  // and for each that is not a plain page inside a document
       auto fetch = [&](int u0) {
         const int u = u0 + lane;
         next_scale = -1.f;
@@ -579,12 +587,14 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
           cur_scale = next_scale;
           cur_ends = next_ends;
           end_mask = __ballot_sync(kAllWarp, cur_ends >= 0);
+          odd_mask = __ballot_sync(kAllWarp, cur_ends >= 0 || cur_scale < 0.f);
           fetch(unit0 + 32);  // also past the stream's end: another stream may go on
         }
         float scales[kUnits];
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) scales[i] = __shfl_sync(kAllWarp, cur_scale, (unit0 + i) & 31);
         const uint32_t ends_here = end_mask >> (unit0 & 31);
+        const bool plain = (odd_mask >> (unit0 & 31) & ((1u << kUnits) - 1u)) == 0;
         bool still_open = open;
         for (int m = 0; m < mt; ++m) {
           float best = bests[m * 32];
@@ -622,10 +632,17 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
               if (lane == 0) mbar_arrive(acce_bar(slot));
             }
             if constexpr (U == 32) {
-              one(b, max_columns<32>(cur));
+              const float v = max_columns<32>(cur);
+              if (plain) best = max_nan(best, v * scales[b]);
+              else one(b, v);
             } else {
-              one(2 * b, max_columns<16>(cur));
-              one(2 * b + 1, max_columns<16>(cur + 16));
+              const float v = max_columns<16>(cur), w = max_columns<16>(cur + 16);
+              if (plain) {
+                best = max3_nan(best, v * scales[2 * b], w * scales[2 * b + 1]);
+              } else {
+                one(2 * b, v);
+                one(2 * b + 1, w);
+              }
             }
           }
           bests[m * 32] = best;
@@ -698,12 +715,21 @@ int launch(const CUtensorMap& map, const PagedArgs& a, cudaStream_t st) {
   const uint32_t smem = smem_layout(NC, a.mt, a.terms, a.kc, a.stages).total;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
     return TMS_ERR_CUDA;
-  kern<<<static_cast<unsigned>(a.groups * a.ranges), kThreads, smem, st>>>(map, a);
-  return cuda_status(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.groups * a.ranges));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = a.packed ? 1 : 0;  // the packing kernel is the launch before
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, map, a));
 }
 
 // Workspace: the chunks' scores of queries of more than 32 rows, then the packed query tiles and
-// their factors when there are several.
+// their factors when there are more than two chunks.
 struct Workspace {
   size_t chunks, packed, factor;
 };
@@ -711,7 +737,7 @@ Workspace workspace_of(int64_t n_queries, int64_t nq, int64_t d, int64_t n_docs)
   Workspace w = {0, 0, 0};
   const int64_t nchunk = (nq + 31) / 32, mtiles = (n_queries * nchunk + 3) / 4;
   if (nchunk > 1) w.chunks = align_up(static_cast<size_t>(n_queries * nchunk * n_docs) * sizeof(float), 128);
-  if (mtiles > 1) {
+  if (n_queries * nchunk > 2) {
     w.packed = static_cast<size_t>(mtiles * 3 * ((d + 127) / 128) * 128) * kRow;
     w.factor = static_cast<size_t>(mtiles) * 128 * sizeof(float);
   }
@@ -807,7 +833,7 @@ extern "C" int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, i
   if (ranges > page_capacity) ranges = page_capacity;
   a.ranges = static_cast<int>(ranges < 1 ? 1 : ranges);
 
-  if (a.n_mtiles > 1) {
+  if (nc == 4) {
     uint8_t* const packed = static_cast<uint8_t*>(workspace) + w.chunks;
     float* const factor = reinterpret_cast<float*>(packed + w.packed);
     paged_pack_kernel<<<static_cast<unsigned>((a.n_mtiles * 128 + 8 * kPackRows - 1) / (8 * kPackRows)), 256, 0, st>>>(
