@@ -418,6 +418,27 @@ def test_scores_other_stream_and_graph(cuda_device):
     assert torch.equal(a(Q), want.cpu())
 
 
+@pytest.mark.parametrize("bq", [1, 2, 9])
+def test_scores_bounded_wait_reports_timeout(bq, cuda_device):
+    """The loads stay out: every wait runs out after the (short) limit, the kernel returns, the host
+    reads the status, and the next call is right."""
+    from tilemaxsim_b200 import _lib, paged_maxsim
+    lib = _lib.load()
+    t, codes, scales, docs = _corpus(RAGGED, 32, 128, 4)
+    Q = _queries(bq, 32, 128, 5, torch.bfloat16)
+    paged_maxsim(Q, codes, scales, t)
+    assert _lib.last_device_error(cuda_device)[0] == _lib.TMS_OK
+    lib.tms_set_debug(50_000_000, 1)
+    try:
+        paged_maxsim(Q, codes, scales, t)
+        rc, word = _lib.last_device_error(cuda_device)
+    finally:
+        lib.tms_set_debug(2_000_000_000, 0)
+    assert rc == _lib.TMS_ERR_TIMEOUT and word & 0x80000000
+    _check_scores(paged_maxsim(Q, codes, scales, t), Q, docs)
+    assert _lib.last_device_error(cuda_device)[0] == _lib.TMS_OK
+
+
 # ------------------------------------------------------------------------------------------ the corpus
 
 def test_corpus_life(cuda_device):
@@ -490,6 +511,13 @@ def test_corpus_life(cuda_device):
         c.add(torch.zeros(5, d).double().cuda(), [5])
     with pytest.raises(IndexError):
         c.remove([11])
+    with pytest.raises(ValueError, match="integers"):
+        c.remove([1.0])
+    with pytest.raises(ValueError, match="integers"):
+        c.add(torch.zeros(5, d).half().cuda(), [5.0])
+    with pytest.raises(ValueError, match="weight"):
+        c.add(torch.zeros(5, d).half().cuda(), [5], norm="rms", weight=torch.ones(d).cuda())
+    c.remove([])
     assert c.n_docs == 11 and all(torch.equal(a, b) for a, b in zip(before, c.tables[:4]))
     c.remove(list(range(11)))
     assert c.n_free == 60 and sorted(c._free.tolist()) == list(range(60))
@@ -499,6 +527,23 @@ def test_corpus_life(cuda_device):
     add([60 * 16], False, 9)
     assert c.n_free == 0
     check()
+
+
+def test_corpus_selection_of_many_short_documents_and_a_long_one(cuda_device):
+    """The longest document's length for each candidate would be far more than the corpus holds."""
+    from tilemaxsim_b200 import PagedCorpus
+    c = PagedCorpus(16, n_pages=3000, max_docs=2100, page_size=16)
+    lengths = [1] * 1000 + [20000] + [3] * 700
+    x = torch.randn(sum(lengths), 16, generator=_rng(1)).half().cuda()
+    c.add(x, torch.tensor(lengths).cuda())
+    ids = torch.randint(-5, 1710, (5000,), generator=_rng(2))
+    ids[ids == 1000] = 7  # the long one is no candidate
+    t = c.select(ids.cuda(), slots=True)
+    assert t.slots.numel() == sum(lengths[i] if 0 <= i < 1701 else 0 for i in ids.tolist())
+    Q = _queries(2, 4, 16, 5, torch.float16)
+    full, got = c.score_queries(Q), c.score_queries(Q, ids.cuda())
+    real = (ids >= 0) & (ids < 1701)
+    assert torch.equal(got[:, real.cuda()], full[:, ids[real].cuda()]) and torch.isinf(got[:, ~real.cuda()]).all()
 
 
 def test_corpus_captured_search_sees_removals(cuda_device):

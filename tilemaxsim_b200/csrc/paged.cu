@@ -513,7 +513,7 @@ __device__ __forceinline__ void exact_row(const PageRows<T, SUM, WEIGHT, STAGED>
 }
 
 template <typename T, bool SUM, bool WEIGHT, bool STAGED>
-__global__ void __launch_bounds__(write_threads<T, SUM, STAGED>(), 1024 / write_threads<T, SUM, STAGED>())
+__global__ void __launch_bounds__(write_threads<T, SUM, STAGED>(), 768 / write_threads<T, SUM, STAGED>())
 page_write_kernel(const WriteArgs a, int group) {
   constexpr int kWriteThreads = write_threads<T, SUM, STAGED>();
   constexpr uint32_t kAllWarp = 0xffffffffu;

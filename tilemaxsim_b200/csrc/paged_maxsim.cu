@@ -503,8 +503,8 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
                 if (terms == 3) mma_f8(tmem + slot * kCols, ad + 2 * term_step, bd, idesc, 1, leader);
               } else {
                 mma_f8_ws<0>(tmem + slot * kCols, ad, bd, idesc, acc, leader);
-                if (terms == 3) mma_f8_ws<1>(tmem + slot * kCols, ad + 2 * term_step, bd, idesc, 1, leader);
-                mma_f8_ws<2>(tmem + slot * kCols, ad + term_step, bd, idesc, 1, leader);
+                if (terms == 3) mma_f8_ws<1>(tmem + slot * kCols, ad + term_step, bd, idesc, 1, leader);
+                mma_f8_ws<2>(tmem + slot * kCols, ad + (terms == 3 ? 2 * term_step : term_step), bd, idesc, 1, leader);
               }
               acc = 1;
             }

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 from typing import NamedTuple
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -154,7 +155,7 @@ def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales:
 
     x: the tokens of all documents (T, d), document i's at token_offsets[i].., or a padded batch
     (n_docs, L, d) whose document i has its tokens in the first rows (lengths must not exceed L);
-    fp16, bf16 or fp32; residual: same shape and dtype. codes and scales are updated in place and
+    fp16, bf16 or fp32; residual: same shape and dtype; weight: (d,) of x's dtype. codes and scales are updated in place and
     returned; pages that the tables do not name keep their content."""
     lib = _lib.load()
     if norm not in _NORMS:
@@ -177,8 +178,8 @@ def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales:
         raise ValueError(f"a padded x has a document for each of the tables' {n_docs}, got {x.shape[0]}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("residual must have the shape and dtype of x")
-    if weight is not None and weight.shape != (d,):
-        raise ValueError(f"weight must be ({d},), got {tuple(weight.shape)}")
+    if weight is not None and (weight.shape != (d,) or weight.dtype != x.dtype):
+        raise ValueError(f"weight must be ({d},) {x.dtype}, got {tuple(weight.shape)} {weight.dtype}")
     rows = 16 // x.element_size()  # elements of 16 bytes
 
     def fits(t):
@@ -189,7 +190,7 @@ def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales:
             x = x.clone(memory_format=torch.contiguous_format)
             residual = None if residual is None else residual.clone(memory_format=torch.contiguous_format)
         if weight is not None:
-            weight = weight.to(x.dtype).contiguous()
+            weight = weight.contiguous()
             weight = weight if weight.data_ptr() % 16 == 0 else weight.clone()
         rc = lib.tms_page_write(
             _ptr(x), _lib.DTYPE_CODE[x.dtype], x.shape[-2], x.stride(0) if padded else 0, x.stride(-2), int(padded),
@@ -289,13 +290,10 @@ class PagedCorpus:
         self._page_docs = torch.full((n_pages,), -1, dtype=torch.int32, device=device)
         # free pages, the next ones to give out at the end
         self._free = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=device)
-        self._host_lengths: list[int] = []
+        self._host_lengths = np.zeros(max_docs, dtype=np.int64)
+        self._longest = self._n_tokens = 0  # a bound on the lengths, and their sum
+        self.n_docs = 0  # documents added so far, removed ones included
         self.n_free = n_pages
-
-    @property
-    def n_docs(self) -> int:
-        """Documents added so far, removed ones included."""
-        return len(self._host_lengths)
 
     @property
     def tables(self) -> PageTables:
@@ -303,21 +301,24 @@ class PagedCorpus:
         n = self.n_docs
         return PageTables(self._page_offsets[:n + 1], self._page_ids, self._page_docs, self._token_offsets[:n + 1], None)
 
-    def _pages_of(self, lengths) -> int:
-        return sum((n + self.page_size - 1) // self.page_size for n in lengths)
+    def _pages_of(self, lengths: np.ndarray) -> int:
+        return int(((lengths + self.page_size - 1) // self.page_size).sum())
 
     def add(self, x: torch.Tensor, lengths: torch.Tensor | list[int], *, residual: torch.Tensor | None = None,
             weight: torch.Tensor | None = None, norm: str = "l2", eps: float | None = None) -> torch.Tensor:
         """Adds documents of the given lengths, their tokens in x as page_write takes them (ragged
         (T, d) or padded (n, L, d)). Returns their ids (n,) int64. Raises ValueError, with the corpus
         as it was, when the pool or the document table has no room."""
-        host = [int(n) for n in (lengths.tolist() if isinstance(lengths, torch.Tensor) else lengths)]
-        n, n_tok, first = len(host), sum(host), self.n_docs
-        if any(m < 0 for m in host):
+        host = np.asarray(lengths.tolist() if isinstance(lengths, torch.Tensor) else lengths)
+        if host.ndim != 1 or (host.size and host.dtype.kind not in "iu"):
+            raise ValueError(f"lengths must be a 1-D list or tensor of integers, got {host.dtype} {host.shape}")
+        host = host.astype(np.int64)
+        n, n_tok, first = host.size, int(host.sum()), self.n_docs
+        if n and host.min() < 0:
             raise ValueError("lengths must not be negative")
         if x.dim() == 2 and x.shape[0] != n_tok:
             raise ValueError(f"x has {x.shape[0]} tokens, the lengths sum to {n_tok}")
-        if x.dim() == 3 and (x.shape[0] != n or max(host, default=0) > x.shape[1]):
+        if x.dim() == 3 and (x.shape[0] != n or host.max(initial=0) > x.shape[1]):
             raise ValueError(f"lengths do not fit a padded batch of shape {tuple(x.shape)}")
         need = self._pages_of(host)
         if need > self.n_free:
@@ -328,7 +329,7 @@ class PagedCorpus:
         if n == 0:
             return ids
         with torch.cuda.device(self.device):
-            dev_lengths = torch.tensor(host, dtype=torch.int64, device=self.device)
+            dev_lengths = torch.from_numpy(host).to(self.device)
             free = self._free[self.n_free - need:self.n_free].flip(0)
             t = page_tables(dev_lengths, self.page_size, free, n_tok, slots=False)
             page_write(x, t, self.codes, self.scales, residual=residual, weight=weight, norm=norm, eps=eps)
@@ -340,27 +341,33 @@ class PagedCorpus:
             self._token_offsets[first + 1:first + 1 + n] = t.token_offsets[1:] + self._token_offsets[first]
             self._token_offsets[first + 1 + n:] = self._token_offsets[first + n].clone()
             self._lengths[first:first + n] = dev_lengths
-        self._host_lengths += host
+        self._host_lengths[first:first + n] = host
+        self._longest = max(self._longest, int(host.max()))
+        self._n_tokens += n_tok
+        self.n_docs += n
         self.n_free -= need
         return ids
 
-    def _host_ids(self, doc_ids: torch.Tensor | list[int]) -> list[int]:
-        ids = [int(i) for i in (doc_ids.tolist() if isinstance(doc_ids, torch.Tensor) else doc_ids)]
-        if any(i < 0 or i >= self.n_docs for i in ids):
+    def _host_ids(self, doc_ids: torch.Tensor | list[int]) -> np.ndarray:
+        ids = np.asarray(doc_ids.tolist() if isinstance(doc_ids, torch.Tensor) else doc_ids)
+        if ids.ndim != 1 or (ids.size and ids.dtype.kind not in "iu"):
+            raise ValueError(f"document ids must be a 1-D list or tensor of integers, got {ids.dtype} {ids.shape}")
+        if ids.size and (ids.min() < 0 or ids.max() >= self.n_docs):
             raise IndexError(f"document ids must be in [0, {self.n_docs})")
-        return ids
+        return ids.astype(np.int64)
 
     def remove(self, doc_ids: torch.Tensor | list[int]) -> None:
         """Removes documents and frees their pages. An id may come twice; a document that is removed
         already, or empty, is left as it is."""
-        ids = sorted({i for i in self._host_ids(doc_ids) if self._host_lengths[i] > 0})
-        if not ids:
+        ids = np.unique(self._host_ids(doc_ids))
+        ids = ids[self._host_lengths[ids] > 0]
+        if not ids.size:
             return
-        freed = self._pages_of(self._host_lengths[i] for i in ids)
+        freed = self._pages_of(self._host_lengths[ids])
         used = self.n_pages - self.n_free
         with torch.cuda.device(self.device):
             gone = torch.zeros(self.max_docs, dtype=torch.bool, device=self.device)
-            gone[torch.tensor(ids, device=self.device)] = True
+            gone[torch.from_numpy(ids).to(self.device)] = True
             out = gone[self._page_docs[:used].long()]
             pages, docs = self._page_ids[:used].clone(), self._page_docs[:used].clone()
             self._free[self.n_free:self.n_free + freed] = pages[out]
@@ -372,16 +379,20 @@ class PagedCorpus:
             shift = self.page_size - 1
             self._page_offsets[1:] = torch.cumsum((self._lengths + shift) // self.page_size, 0)
             self._token_offsets[1:] = torch.cumsum(self._lengths, 0)
-        for i in ids:
-            self._host_lengths[i] = 0
+        self._n_tokens -= int(self._host_lengths[ids].sum())
+        self._host_lengths[ids] = 0
         self.n_free += freed
 
     def select(self, doc_ids: torch.Tensor, n_tokens: int | None = None, slots: bool = False) -> PageTables:
         """The tables of the given documents (an id outside the corpus is an empty document).
-        n_tokens bounds their tokens; by default the longest document's length for each."""
+        n_tokens bounds their tokens. By default it is the longest document's length for each, and
+        where that is far more than the corpus holds, their own sum, for which the host waits."""
         doc_ids = _ints(doc_ids, torch.int64, "doc_ids")
         if n_tokens is None:
-            n_tokens = doc_ids.numel() * max(self._host_lengths, default=0)
+            n_tokens = doc_ids.numel() * self._longest
+            if n_tokens > max(4 * self._n_tokens, 1 << 24):
+                inside = (doc_ids >= 0) & (doc_ids < self.n_docs)
+                n_tokens = int(self._lengths[doc_ids.clamp(0, self.max_docs - 1)][inside].sum())
         n = self.n_docs
         return select_page_tables(self._lengths[:n], self.page_size, self._page_offsets[:n + 1], self._page_ids, doc_ids,
                                   n_tokens, slots=slots)
@@ -405,6 +416,5 @@ class PagedCorpus:
         """The stored tokens of the given documents: (T, d) values and (n + 1,) int64 offsets, the
         layout maxsim_batched and save_shard take."""
         ids = self._host_ids(doc_ids)
-        n_tok = sum(self._host_lengths[i] for i in ids)
-        t = self.select(torch.tensor(ids, dtype=torch.int64, device=self.device), n_tok, slots=True)
+        t = self.select(torch.from_numpy(ids).to(self.device), int(self._host_lengths[ids].sum()), slots=True)
         return page_read(self.codes, self.scales, t.slots, dtype), t.token_offsets
