@@ -307,7 +307,8 @@ TMS_API int tms_page_read(const void* codes, const float* scales, int64_t n_page
                           int64_t page_size, int64_t d, const int64_t* slots, int64_t n_slots,
                           void* out, int out_dtype, void* stream);
 
-TMS_API size_t tms_paged_workspace_size(int64_t n_queries, int64_t nq, int64_t d, int64_t n_docs);
+TMS_API size_t tms_paged_workspace_size(int64_t n_queries, int64_t nq, int64_t d, int64_t n_docs,
+                                        int64_t page_size, int64_t page_capacity);
 
 /* out[q * n_docs + i] = sum_t max over the values v of document i's pages of <Q[q,t,:], v> (fp32
  * accumulation); a document without pages scores -inf, one with a NaN page NaN. Q: (n_queries, nq,

@@ -131,7 +131,7 @@ def test_c_abi_refusals_without_gpu():
     assert score(Q=odd) == score(codes=odd) == L.TMS_ERR_INVALID
     assert score(d=40) == score(d=512) == score(page=48) == score(pages=1 << 27) == L.TMS_ERR_UNSUPPORTED
     assert score(nb=0) == score(n=0) == L.TMS_OK
-    need = lib.tms_paged_workspace_size(1, 64, 128, 2)
+    need = lib.tms_paged_workspace_size(1, 64, 128, 2, 32, 4)
     if need:
         assert score(nq=64, ws=nul) == score(nq=64, wsb=need - 1) == L.TMS_ERR_WORKSPACE
 

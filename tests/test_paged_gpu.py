@@ -322,6 +322,23 @@ def test_scores_long_documents(cuda_device):
     _check_scores(paged_maxsim(Q, codes, scales, t), Q, docs)
 
 
+@pytest.mark.parametrize("lengths", [[5000], [100000], [1500, 1], [3000, 2000, 0, 9000, 1], list(range(1000, 3000, 37)),
+                                     [4000] * 3 + [0] * 5 + [17] * 2])
+@pytest.mark.parametrize("bq,nq,d,page,dtype", [(1, 32, 128, 32, torch.bfloat16), (2, 20, 64, 16, torch.float16),
+                                                 (1, 70, 128, 128, torch.float16), (9, 32, 256, 64, torch.bfloat16),
+                                                 (21, 32, 128, 32, torch.bfloat16)])
+def test_scores_documents_over_several_ranges(bq, nq, d, page, dtype, lengths, cuda_device):
+    """Few long documents are cut over the whole GPU and joined again."""
+    from tilemaxsim_b200 import paged_maxsim
+    if d * sum(lengths) > 13_000_000:
+        lengths = [n // 2 for n in lengths]
+    t, codes, scales, docs = _corpus(lengths, page, d, 1)
+    Q = _queries(bq, nq, d, 3, dtype)
+    got = paged_maxsim(Q, codes, scales, t)
+    _check_scores(got, Q, docs)
+    assert torch.equal(got, paged_maxsim(Q, codes, scales, t))
+
+
 @pytest.mark.parametrize("bq,page", [(1, 32), (2, 16), (4, 64), (20, 32)])
 def test_scores_long_streams(bq, page, cuda_device):
     """Enough documents that every part of the corpus takes many steps, and parts end at different ones:

@@ -69,7 +69,7 @@ SIGNATURES = {
     "tms_page_write": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _i32, ctypes.c_float, _i64, _i64, _vp,
                               _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _vp]),
     "tms_page_read": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _i32, _vp]),
-    "tms_paged_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
+    "tms_paged_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "tms_paged_maxsim": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp,
                                 _vp, _sz, _vp]),
     "tms_topk_workspace_size": (_sz, [_i64, _i64, _i64]),

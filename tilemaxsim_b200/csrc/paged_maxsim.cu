@@ -21,7 +21,9 @@
 // 100k documents: 549 us with the rows repeated by hand at M = 128, 421 us so). Either way each of
 // the eight epilogue warps reads one chunk's rows against one stream's columns and keeps each row's
 // running maximum. A document cut by a stream boundary is joined from the streams' partial maxima
-// when the CTA is done. No merge between CTAs, no atomic: results do not depend on the launch.
+// when the CTA is done. Few long documents would leave ranges uneven: they are cut evenly instead, and
+// what a document has in several ranges is joined by a kernel of its own. No atomics, and the sums
+// run in one order: results do not depend on the launch.
 //
 // Warp roles (320 threads, one CTA an SM): warp 0 loads pages by TMA (a lane for each box of up to
 // 32 rows), warp 1 owns TMEM and issues the MMAs, warps 2-9 are the epilogue. A document that ends
@@ -49,6 +51,12 @@ constexpr int kQueue = 16;        // documents of an epilogue warp's queue
 constexpr int kQueueStride = 33;  // floats; the odd stride keeps both accesses conflict-free
 constexpr int kMostMt = 4;        // most M tiles of a CTA
 constexpr float kNegInf = -__builtin_huge_valf();
+// What a range begins with: nothing of its own, a document's first page, or a page inside a document
+// that goes on behind the range.
+constexpr int kRangeEmpty = -3, kRangeClean = -2, kRangeInside = -1;
+constexpr int kSplitTokens = 1024;  // ranges cut documents whose mean length is this or more
+constexpr int kSplitDocs = 16;      // and of which there are fewer than this for each range
+constexpr int kMostSms = 160;       // CTAs that the workspace has parts for
 
 struct PagedArgs {
   const void* Q;
@@ -69,6 +77,11 @@ struct PagedArgs {
   const int32_t* page_docs;
   int64_t n_docs, page_cap;
   float* out;          // (n_chunks, n_docs)
+  // Where ranges may cut documents: (ranges, 2, 4 n_mtiles, 32) row maxima of the document that a
+  // range begins in the middle of, and of the one that it ends in the middle of; and (ranges, 2)
+  // which document the first one is (kRange...) and whether there is a second one. Else nullptr.
+  float* parts;
+  int* part_docs;
   uint32_t* err;
   uint64_t timeout_ns;
   int debug_flags;
@@ -77,7 +90,7 @@ struct PagedArgs {
 struct Stream {  // what one stream of a CTA covers
   int32_t first, units;  // first table entry; boxes
   int32_t open;          // whether its first document began in the stream before
-  int32_t end;           // the CTA's last table entry + 1
+  int32_t end;           // the last table entry + 1 that a document can reach
 };
 struct SmemLayout {
   uint32_t q, q_bytes, stage, queue, best, head, factor, bars, streams, misc, total;
@@ -321,6 +334,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
 
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + L.misc);
   int* const tiles = reinterpret_cast<int*>(smem + L.misc + 4);
+  int* const goes_on = reinterpret_cast<int*>(smem + L.misc + 48);
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + L.misc + 8);
   volatile int* const never_flag = reinterpret_cast<volatile int*>(smem + L.misc + 12);
   int* const head_docs = reinterpret_cast<int*>(smem + L.misc + 16);  // 8: an epilogue warp's head document
@@ -353,7 +367,9 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       fence_mbar_init();
     }
     const int64_t total = clamp_entry(a, __ldg(a.page_offsets + a.n_docs));
-    const int64_t cut = lane < 2 ? cut_at(a, total, range + lane, a.ranges) : 0;
+    const int64_t cut = lane >= 2   ? 0
+                        : a.parts ? total * (range + lane) / a.ranges
+                                  : cut_at(a, total, range + lane, a.ranges);
     const int64_t lo = __shfl_sync(kAllWarp, cut, 0);
     int64_t hi = __shfl_sync(kAllWarp, cut, 1);
     hi = hi < lo ? lo : hi;
@@ -361,8 +377,8 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
     const int64_t next = lo + (hi - lo) * (lane + 1) / kStreams;
     const int units = lane < kStreams ? static_cast<int>((next - first) << a.unit_shift) : 0;  // below 2^30 (host)
     if (lane < kStreams) {
-      const bool open = lane > 0 && units > 0 && first > lo && __ldg(a.page_docs + first) == __ldg(a.page_docs + first - 1);
-      streams[lane] = Stream{static_cast<int32_t>(first), units, open, static_cast<int32_t>(hi)};
+      const bool open = units > 0 && first > (a.parts ? 0 : lo) && __ldg(a.page_docs + first) == __ldg(a.page_docs + first - 1);
+      streams[lane] = Stream{static_cast<int32_t>(first), units, open, static_cast<int32_t>(a.parts ? total : hi)};
     }
     n_tiles = (units + kUnits - 1) / kUnits;
 #pragma unroll
@@ -370,7 +386,11 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       const int y = __shfl_xor_sync(kAllWarp, n_tiles, o);
       n_tiles = y > n_tiles ? y : n_tiles;
     }
-    if (lane == 0) *tiles = n_tiles;
+    if (lane == 0) {
+      *tiles = n_tiles;
+      // whether the last document goes on in the next range
+      *goes_on = a.parts && hi > lo && hi < total && __ldg(a.page_docs + hi) == __ldg(a.page_docs + hi - 1);
+    }
     __syncwarp();
     dead = *abort_flag != 0;
     asm volatile("barrier.arrive %0, %1;" ::"r"(kReadyBarrier), "r"(kThreads) : "memory");
@@ -419,6 +439,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
     // no role runs: misaligned shared memory
   } else if (n_tiles == 0) {
     if (warp >= kEpiWarp0) write_empty();
+    if (a.parts && threadIdx.x == 32) a.part_docs[2 * range] = kRangeEmpty;
   } else if (warp == 0) {
     // ------------------------------------------------------------------ loads: a lane for each box
     static_assert(kTile / U <= 32, "a lane for each box");
@@ -654,23 +675,41 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       // Documents that streams share: the chunk's first stream's warp walks the streams in order.
       asm volatile("barrier.sync %0, %1;" ::"r"(kJoinBarrier), "r"(256) : "memory");
       if (ok && quarter < NC && half == 0) {
+        int begins = kRangeClean;
         for (int m = 0; m < mt; ++m) {
+          float* const part = a.parts + (static_cast<int64_t>(range) * 8 * a.n_mtiles + first_chunk + m * 4) * 32 + lane;
+          const float f = factor[m * 32 * NC];
           float run = kNegInf;
+          bool first = true, inside = false;  // inside: still in the document that the range began in the middle of
           for (int s = 0; s < kStreams; ++s) {
             if (streams[s].units == 0) continue;
             const int at = (s & 1) * 4 + (s >> 1) * NC + chunk;
             const float tail = reinterpret_cast<const float*>(smem + L.best)[(at * a.mt + m) * 32 + lane];
+            if (first) inside = streams[s].open;
+            first = false;
             if (streams[s].open && head_docs[at] < 0) {  // inside one document from end to end
               run = max_nan(run, tail);
               continue;
             }
             if (streams[s].open) {
-              push(m, head_docs[at],
-                   max_nan(run, reinterpret_cast<const float*>(smem + L.head)[(at * a.mt + m) * 32 + lane]));
-              if (queued == kQueue) flush();
+              const float v = max_nan(run, reinterpret_cast<const float*>(smem + L.head)[(at * a.mt + m) * 32 + lane]);
+              if (inside) {
+                part[0] = v * f;
+                begins = head_docs[at];
+                inside = false;
+              } else {
+                push(m, head_docs[at], v);
+                if (queued == kQueue) flush();
+              }
             }
             run = tail;
           }
+          if (inside) begins = kRangeInside;
+          if (*goes_on) part[4 * a.n_mtiles * 32] = run * f;
+        }
+        if (a.parts && chunk == 0 && lane == 0) {
+          a.part_docs[2 * range] = begins;
+          a.part_docs[2 * range + 1] = *goes_on;
         }
       }
       if (queued) flush();
@@ -682,6 +721,37 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(*tmem_slot, 512);
+  }
+}
+
+// Documents that several ranges have parts of: a warp for each range that one begins in, and chunk.
+// The sum runs as the scoring kernel's: rows 0-15, rows 16-31, then both.
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
+  const int lane = lane_id();
+  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int r = static_cast<int>(w / a.n_chunks), chunk = static_cast<int>(w % a.n_chunks);
+  if (r >= a.ranges) return;
+  const int64_t step = static_cast<int64_t>(4) * a.n_mtiles * 32;  // from a range's first part to its second
+  const float* const at = a.parts + static_cast<int64_t>(chunk) * 32 + lane;
+  const int begins = a.part_docs[2 * r];
+  if (begins == kRangeEmpty || begins == kRangeInside || !a.part_docs[2 * r + 1]) return;
+  float v = at[(2 * r + 1) * step];
+  for (int e = r + 1; e < a.ranges; ++e) {
+    const int doc = a.part_docs[2 * e];
+    if (doc == kRangeEmpty) continue;
+    if (doc == kRangeInside) {
+      v = max_nan(v, at[(2 * e + 1) * step]);
+      continue;
+    }
+    if (doc < 0 || doc >= a.n_docs) return;
+    v = max_nan(v, at[2 * e * step]);
+    float lo = __shfl_sync(0xffffffffu, v, 0), hi = __shfl_sync(0xffffffffu, v, 16);
+    for (int i = 1; i < 16; ++i) {
+      lo += __shfl_sync(0xffffffffu, v, i);
+      hi += __shfl_sync(0xffffffffu, v, 16 + i);
+    }
+    if (lane == 0) a.out[chunk * a.n_docs + doc] = lo + hi;
+    return;
   }
 }
 
@@ -729,17 +799,24 @@ int launch(const CUtensorMap& map, const PagedArgs& a, cudaStream_t st) {
 }
 
 // Workspace: the chunks' scores of queries of more than 32 rows, then the packed query tiles and
-// their factors when there are more than two chunks.
+// their factors when there are more than two chunks, then the parts of documents cut by ranges.
 struct Workspace {
-  size_t chunks, packed, factor;
+  size_t chunks, packed, factor, parts, part_docs;
+  size_t total() const { return chunks + packed + factor + parts + part_docs; }
 };
-Workspace workspace_of(int64_t n_queries, int64_t nq, int64_t d, int64_t n_docs) {
-  Workspace w = {0, 0, 0};
+Workspace workspace_of(int64_t n_queries, int64_t nq, int64_t d, int64_t n_docs, int64_t page_size, int64_t page_cap) {
+  Workspace w = {};
   const int64_t nchunk = (nq + 31) / 32, mtiles = (n_queries * nchunk + 3) / 4;
   if (nchunk > 1) w.chunks = align_up(static_cast<size_t>(n_queries * nchunk * n_docs) * sizeof(float), 128);
   if (n_queries * nchunk > 2) {
     w.packed = static_cast<size_t>(mtiles * 3 * ((d + 127) / 128) * 128) * kRow;
     w.factor = static_cast<size_t>(mtiles) * 128 * sizeof(float);
+  }
+  // Mean lengths by the table's capacity, which is all the host knows. Ranges times M tiles are at
+  // most 4 for each SM (a CTA holds up to four M tiles).
+  if (mtiles <= 2 * kMostSms && page_cap * page_size >= n_docs * kSplitTokens && n_docs < kSplitDocs * kMostSms) {
+    w.parts = static_cast<size_t>(4 * kMostSms + mtiles) * 8 * 32 * sizeof(float);
+    w.part_docs = 2 * kMostSms * sizeof(int);
   }
   return w;
 }
@@ -749,10 +826,10 @@ Workspace workspace_of(int64_t n_queries, int64_t nq, int64_t d, int64_t n_docs)
 
 using namespace tms;
 
-extern "C" size_t tms_paged_workspace_size(int64_t n_queries, int64_t nq, int64_t d, int64_t n_docs) {
-  if (n_queries <= 0 || nq <= 0 || d <= 0 || n_docs <= 0) return 0;
-  const Workspace w = workspace_of(n_queries, nq, d, n_docs);
-  return w.chunks + w.packed + w.factor;
+extern "C" size_t tms_paged_workspace_size(int64_t n_queries, int64_t nq, int64_t d, int64_t n_docs,
+                                           int64_t page_size, int64_t page_capacity) {
+  if (n_queries <= 0 || nq <= 0 || d <= 0 || n_docs <= 0 || page_size <= 0 || page_capacity <= 0) return 0;
+  return workspace_of(n_queries, nq, d, n_docs, page_size, page_capacity).total();
 }
 
 extern "C" int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, int64_t nq,
@@ -781,8 +858,9 @@ extern "C" int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, i
   if ((reinterpret_cast<uintptr_t>(Q) & 15) || (reinterpret_cast<uintptr_t>(codes) & 15) ||
       (reinterpret_cast<uintptr_t>(workspace) & 127))
     return TMS_ERR_INVALID;
-  const Workspace w = workspace_of(n_queries, nq, d, n_docs);
-  const size_t need = w.chunks + w.packed + w.factor;
+  const Workspace w =
+      page_capacity > 0 ? workspace_of(n_queries, nq, d, n_docs, page_size, page_capacity) : Workspace{};
+  const size_t need = w.total();
   if (need && (!workspace || workspace_bytes < need)) return TMS_ERR_WORKSPACE;
   int status = TMS_OK;
   const DeviceInfo* dev = current_device_info(&status);
@@ -833,9 +911,13 @@ extern "C" int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, i
   if (ranges > page_capacity) ranges = page_capacity;
   a.ranges = static_cast<int>(ranges < 1 ? 1 : ranges);
 
+  uint8_t* const packed = static_cast<uint8_t*>(workspace) + w.chunks;
+  float* const factor = reinterpret_cast<float*>(packed + w.packed);
+  if (w.parts && ranges > 1 && dev->num_sms <= kMostSms && n_docs < kSplitDocs * ranges) {
+    a.parts = factor + w.factor / sizeof(float);
+    a.part_docs = reinterpret_cast<int*>(a.parts + w.parts / sizeof(float));
+  }
   if (nc == 4) {
-    uint8_t* const packed = static_cast<uint8_t*>(workspace) + w.chunks;
-    float* const factor = reinterpret_cast<float*>(packed + w.packed);
     paged_pack_kernel<<<static_cast<unsigned>((a.n_mtiles * 128 + 8 * kPackRows - 1) / (8 * kPackRows)), 256, 0, st>>>(
         a, packed, factor);
     if (cudaGetLastError() != cudaSuccess) return TMS_ERR_CUDA;
@@ -849,7 +931,12 @@ extern "C" int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, i
   if (rc != TMS_OK) return rc;
   if (U == 16) rc = nc == 1 ? launch<1, 16>(map, a, st) : nc == 2 ? launch<2, 16>(map, a, st) : launch<4, 16>(map, a, st);
   else rc = nc == 1 ? launch<1, 32>(map, a, st) : nc == 2 ? launch<2, 32>(map, a, st) : launch<4, 32>(map, a, st);
-  if (rc != TMS_OK || nchunk == 1) return rc;
+  if (rc != TMS_OK) return rc;
+  if (a.parts) {
+    paged_join_kernel<<<static_cast<unsigned>((static_cast<int64_t>(a.ranges) * a.n_chunks + 7) / 8), 256, 0, st>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return TMS_ERR_CUDA;
+  }
+  if (nchunk == 1) return TMS_OK;
   paged_sum_kernel<<<blocks_for(n_queries * n_docs, dev), 256, 0, st>>>(a.out, out, n_queries, n_docs, a.nchunk);
   return cuda_status(cudaGetLastError());
 }

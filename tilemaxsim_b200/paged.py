@@ -246,7 +246,7 @@ def paged_maxsim(Qb: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, ta
         Qb = Qb if Qb.data_ptr() % 16 == 0 else Qb.clone()
         out = torch.empty((Bq, n_docs), dtype=torch.float32, device=dev)
         if Bq > 0 and n_docs > 0:
-            ws_bytes = lib.tms_paged_workspace_size(Bq, Nq, d, n_docs)
+            ws_bytes = lib.tms_paged_workspace_size(Bq, Nq, d, n_docs, page_size, tables.page_ids.numel())
             ws, ws_ptr = _lib.workspace(ws_bytes, dev, align=256)
             rc = lib.tms_paged_maxsim(
                 _ptr(Qb), _lib.DTYPE_CODE[Qb.dtype], Bq, Nq, d, _ptr(codes), _ptr(scales), n_pages, page_size,
