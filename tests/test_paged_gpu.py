@@ -339,6 +339,22 @@ def test_scores_documents_over_several_ranges(bq, nq, d, page, dtype, lengths, c
     assert torch.equal(got, paged_maxsim(Q, codes, scales, t))
 
 
+@pytest.mark.parametrize("d", [16, 32, 48, 80, 112, 144, 176, 240])
+@pytest.mark.parametrize("bq,page,dtype", [(1, 16, torch.float16), (2, 32, torch.bfloat16), (3, 16, torch.bfloat16),
+                                            (19, 32, torch.float16), (40, 16, torch.bfloat16)])
+def test_scores_token_widths(bq, page, dtype, d, cuda_device):
+    """Every kind of width, through enough documents that every stage is used several times."""
+    from tilemaxsim_b200 import paged_maxsim
+    lengths = torch.randint(0, 150, (1200,), generator=_rng(d)).tolist()
+    t, codes, scales, docs = _corpus(lengths, page, d, 1)
+    Q = _queries(bq, 32, d, 3, dtype)
+    got = paged_maxsim(Q, codes, scales, t)
+    pick = torch.randperm(1200, generator=_rng(2))[:200].tolist()
+    _check_scores(got[:, pick], Q, [docs[i] for i in pick])
+    for i in range(0, bq, 7):  # alone or in a batch: within the bound of the kernel's own arithmetic
+        _check_scores(paged_maxsim(Q[i:i + 1], codes, scales, t)[:, pick], Q[i:i + 1], [docs[j] for j in pick])
+
+
 @pytest.mark.parametrize("bq,page", [(1, 32), (2, 16), (4, 64), (20, 32)])
 def test_scores_long_streams(bq, page, cuda_device):
     """Enough documents that every part of the corpus takes many steps, and parts end at different ones:

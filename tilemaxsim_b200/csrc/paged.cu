@@ -157,6 +157,9 @@ __device__ __forceinline__ int64_t owner_of(const int64_t* page_offsets, int64_t
   return lo;
 }
 
+// 400,000 documents (72.8M slots, 582 MB) take 125 us here and 12 us for their offsets; a plain fill
+// of the slots takes 81 us. A slot at a time with its own bounds checks took 219 us.
+//
 // Page ids, owners and slots of the 32 table entries from k0 on, by one warp: a lane for each entry
 // (`doc` owns it, where it lies below the total), then the entries' slots one after the other. The
 // entries' tokens follow one another, so one base and 32-bit distances from it place them.
@@ -412,8 +415,9 @@ struct Eight {
 // elements) are done again in fp64. Pages that hold a magnitude or a sum of squares outside [1e-30,
 // 1e30], zeros apart, go through fp64 altogether; NaN and infinities are found there.
 //
-// 20,000 documents (3.6M tokens, 128 bf16 values, unit length), in us: rows held in registers, all
-// sums in fp64 600-820, in fp32 770 (few warps fit); see the launch for what this form takes.
+// 20,000 documents (3.6M tokens, 128 bf16 values, unit length) take 530 us, 2.7 TB/s: issue slots
+// (64% busy), not memory, bound it. Rows held in registers took 770 us (few warps fit), all sums in
+// fp64 600-820, sixteen elements a lane 546, fp64 roots for the rows that set the scale 830.
 __device__ __forceinline__ double max_keep_nan(double x, double y) { return y <= x || x != x ? x : y; }
 __device__ __forceinline__ bool usual(float v) { return v >= 1e-30f && v <= 1e30f; }
 
@@ -819,9 +823,10 @@ struct ReadArgs {
 
 // out[t] = scale * code of slot t; a slot outside the pool gives a row of zeros. One multiplication
 // in fp32, then one rounding to the output type. A group of lanes takes a row, sixteen elements a
-// lane (one 16-byte load), and a thread four rows, whose loads are all in flight before the first
-// store: what bounds it is memory. The output is written past the caches' working set.
-constexpr int kReadRows = 4;
+// lane (one 16-byte load), and a thread ROWS rows, whose loads are all in flight before the first
+// store: what bounds it is memory. The output is written past the caches' working set. 3.6M rows of
+// 128 to bf16 take 253 us with two rows and 235 us with four (5.8 TB/s), 182 thousand to fp16 take
+// 12.6 and 14.9 us: four where that makes eight CTAs an SM and more, two below.
 
 template <typename T>
 __device__ __forceinline__ uint32_t two_as(float x, float y) {
@@ -839,23 +844,23 @@ __device__ __forceinline__ float2 e4m3x2_value(uint32_t two) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-template <typename T>
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(256) page_read_kernel(const ReadArgs a, int group) {
   const int sub = threadIdx.x & (group - 1);
   const int64_t rows = 256 / group;  // of a CTA at a time
   const bool in_row = sub * 16 < a.d;
-  for (int64_t t0 = blockIdx.x * rows * kReadRows + threadIdx.x / group; t0 < a.n_slots;
-       t0 += gridDim.x * rows * kReadRows) {
-    int64_t slot[kReadRows];
-    uint4 c[kReadRows];
-    float scale[kReadRows];
+  for (int64_t t0 = blockIdx.x * rows * ROWS + threadIdx.x / group; t0 < a.n_slots;
+       t0 += gridDim.x * rows * ROWS) {
+    int64_t slot[ROWS];
+    uint4 c[ROWS];
+    float scale[ROWS];
 #pragma unroll
-    for (int i = 0; i < kReadRows; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       const int64_t t = t0 + i * rows;
       slot[i] = t < a.n_slots ? __ldg(a.slots + t) : -1;
     }
 #pragma unroll
-    for (int i = 0; i < kReadRows; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       c[i] = make_uint4(0, 0, 0, 0);
       scale[i] = 0.f;
       if (slot[i] >= 0 && (slot[i] >> a.page_shift) < a.n_pages && in_row) {
@@ -864,7 +869,7 @@ __global__ void __launch_bounds__(256) page_read_kernel(const ReadArgs a, int gr
       }
     }
 #pragma unroll
-    for (int i = 0; i < kReadRows; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
       const int64_t t = t0 + i * rows;
       if (t >= a.n_slots || !in_row) continue;
       const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
@@ -889,6 +894,19 @@ __global__ void __launch_bounds__(256) page_read_kernel(const ReadArgs a, int gr
       }
     }
   }
+}
+
+template <typename T>
+void launch_read(const ReadArgs& a, const DeviceInfo* dev, cudaStream_t st) {
+  int group = 1;  // lanes of a row
+  while (group * 16 < a.d) group <<= 1;
+  const int64_t rows = 256 / group, most = static_cast<int64_t>(dev->num_sms) * 16;
+  const bool many = a.n_slots >= rows * 4 * dev->num_sms * 8;
+  const int64_t each = rows * (many ? 4 : 2);
+  const int64_t blocks = (a.n_slots + each - 1) / each;
+  const unsigned grid = static_cast<unsigned>(blocks < most ? blocks : most);
+  if (many) page_read_kernel<T, 4><<<grid, 256, 0, st>>>(a, group);
+  else page_read_kernel<T, 2><<<grid, 256, 0, st>>>(a, group);
 }
 
 int page_shift_of(int64_t page_size) {
@@ -1002,16 +1020,9 @@ extern "C" int tms_page_read(const void* codes, const float* scales, int64_t n_p
   if (!dev) return status;
   const ReadArgs a{static_cast<const uint8_t*>(codes), scales, n_pages, shift, static_cast<int>(d), slots,
                    n_slots, out};
-  int group = 1;  // lanes of a row
-  while (group * 16 < d) group <<= 1;
-  const int64_t rows = 256 / group * kReadRows;
-  int64_t blocks = (n_slots + rows - 1) / rows;
-  const int64_t most = static_cast<int64_t>(dev->num_sms) * 16;
-  if (blocks > most) blocks = most;
-  const unsigned grid = static_cast<unsigned>(blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (out_dtype == TMS_F16) page_read_kernel<__half><<<grid, 256, 0, st>>>(a, group);
-  else if (out_dtype == TMS_BF16) page_read_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, group);
-  else page_read_kernel<float><<<grid, 256, 0, st>>>(a, group);
+  if (out_dtype == TMS_F16) launch_read<__half>(a, dev, st);
+  else if (out_dtype == TMS_BF16) launch_read<__nv_bfloat16>(a, dev, st);
+  else launch_read<float>(a, dev, st);
   return cuda_status(cudaGetLastError());
 }

@@ -18,12 +18,20 @@
 // pages. Query rows are the MMA's M dimension, 32 rows (a "chunk") to a TMEM lane quarter. Up to
 // four chunks at a time use M = 128; one or two use the weight-stationary MMA with M = 32 or 64,
 // which repeats the rows over the lane quarters and gives each quarter its own columns (a scan of
-// 100k documents: 549 us with the rows repeated by hand at M = 128, 421 us so). Either way each of
+// 100k documents took 549 us with the rows repeated by hand at M = 128). Either way each of
 // the eight epilogue warps reads one chunk's rows against one stream's columns and keeps each row's
 // running maximum. A document cut by a stream boundary is joined from the streams' partial maxima
 // when the CTA is done. Few long documents would leave ranges uneven: they are cut evenly instead, and
 // what a document has in several ranges is joined by a kernel of its own. No atomics, and the sums
 // run in one order: results do not depend on the launch.
+//
+// What bounds it. One query over 100k documents (18.2M tokens, 2.53 GB of pages): memory, 405 us, 6.2
+// TB/s. 64 queries over 4,000 documents: the tensor cores (87% of their cycles), 245 us, 1,560 TFLOP/s
+// of the query's own products, which the two terms double. 5 queries of 77 rows at d = 256 in fp16
+// (three terms): the tensor cores (92%), 206 us. Pages of 16 rows, or narrow ones, at one to four
+// chunks: the TMA's boxes, about 65 clocks each and 2 a row whatever it holds (d = 64, pages of 16, 5.1M
+// tokens: 146 us); copying them by cp.async took 228 us, the proxy fences waiting for the copies.
+// Under a power cap that lowers the clocks these grow by about a tenth.
 //
 // Warp roles (320 threads, one CTA an SM): warp 0 loads pages by TMA (a lane for each box of up to
 // 32 rows), warp 1 owns TMEM and issues the MMAs, warps 2-9 are the epilogue. A document that ends
@@ -154,7 +162,7 @@ __device__ __forceinline__ uint32_t elect_one() {
 }
 // D(tmem) (+)= A * B^T, both K-major e4m3 in shared memory, fp32 accumulation, issued by the lane
 // whose `leader` is set. The whole warp runs the loop around it: the descriptors then stay in
-// uniform registers (64 queries, 4k documents: 423 us under "lane == 0", 324 us so).
+// uniform registers (64 queries, 4k documents: 423 us under "lane == 0", 324 us so at the time).
 __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                        uint32_t accumulate, uint32_t leader) {
   asm volatile(
