@@ -201,6 +201,17 @@ __device__ __forceinline__ void commit(uint32_t bar, uint32_t leader) {
       "r"(leader)
       : "memory");
 }
+// tma_load_2d by the lane whose `leader` is set; all lanes of a converged warp run it alike.
+__device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y,
+                                         uint64_t policy, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4}], [%2], %5;\n\t}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "l"(policy), "r"(leader)
+      : "memory");
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
@@ -465,6 +476,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
     for (int i = 0; i < kAhead; ++i) ids[i] = page_of(i * kUnits + nth);
     int s = 0;
     uint32_t ph = 0, armed = 0, armed_par = 0;
+    const uint32_t leader = elect_one();
     bool ok = !(a.debug_flags & 1);
     for (int t0 = 0; ok && t0 < n_tiles; t0 += kAhead) {
 #pragma unroll
@@ -475,7 +487,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       const int64_t id = ids[i];
       ids[i] = page_of(unit + kAhead * kUnits);
       const bool load = id >= 0 && id < a.n_pages;
-      const uint32_t boxes = __popc(__ballot_sync(kAllWarp, load));
+      const uint32_t mask = __ballot_sync(kAllWarp, load), boxes = __popc(mask);
       const int32_t y = static_cast<int32_t>(id << a.page_shift) + (unit & half_mask) * U;
       for (int c = 0; c < a.kc; ++c) {
         ok = mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, a.timeout_ns, a.err, 41);
@@ -485,9 +497,13 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
         armed |= 1u << s;
         armed_par = (armed_par & ~(1u << s)) | (ph << s);
         __syncwarp();
-        if (load)
-          tma_load_2d(base + L.stage + static_cast<uint32_t>(s) * kStageBytes + lane * U * kRow, &codes_map,
-                      full_bar(s), c * 128, y, policy);
+#pragma unroll
+        for (int b = 0; b < kTile / U; ++b) {
+          const int yb = __shfl_sync(kAllWarp, y, b);
+          if (mask >> b & 1u)
+            box_load(base + L.stage + static_cast<uint32_t>(s) * kStageBytes + b * U * kRow, &codes_map, full_bar(s),
+                     c * 128, yb, policy, leader);
+        }
         if (++s == a.stages) { s = 0; ph ^= 1u; }
       }
      }
