@@ -257,7 +257,7 @@ TMS_API int tms_topk_merge_packed(const int64_t* gathered, int64_t world, int64_
  * page_tables / select_page_tables / page_write / page_read / paged_maxsim.
  *
  * A pool holds n_pages pages of page_size (16, 32, 64 or 128) token rows: codes (n_pages, page_size,
- * d) e4m3, 16-byte aligned, and scales (n_pages) fp32; a token's value is scale * code. A document
+ * d) e4m3, 16-byte aligned, and scales (n_pages) fp32, not negative; a token's value is scale * code. A document
  * owns ceil(length / page_size) pages: entries [page_offsets[i], page_offsets[i + 1]) of page_ids,
  * in order. page_docs names each entry's document. Rows behind a document's last token repeat that
  * token. d is a multiple of 16, at most TMS_PAGED_MAX_D. Whatever the tables hold, no call reads or

@@ -187,6 +187,31 @@ def test_write_padded_batch_and_strides(dtype, cuda_device):
         np.testing.assert_array_equal(got[1], want[1])
 
 
+def test_write_one_row_of_any_stride(cuda_device):
+    """A dimension of one element may have any stride: a column seen as a row, a broadcast document."""
+    from tilemaxsim_b200 import page_write
+    d, page = 32, 16
+    x = torch.randn(d, generator=_rng(3)).half().cuda()
+    t, n_pages = _layout([1], page, 1)
+
+    def write(v):
+        codes = torch.zeros(n_pages, page, d, device=cuda_device).to(torch.float8_e4m3fn)
+        scales = torch.zeros(n_pages, device=cuda_device)
+        page_write(v, t, codes, scales)
+        return torch.cat([codes.float().flatten(), scales])
+
+    want = write(x[None])
+    for v in (x[:, None].t(), x[:, None].t()[None], x.as_strided((1, 1, d), (3, 5, 1)), x.as_strided((1, d), (7, 1))):
+        assert v.shape[-1] == d and torch.equal(write(v), want)
+    # one token for every row of a padded batch
+    t, n_pages = _layout([3, 2], page, 1)
+    codes = torch.zeros(n_pages, page, d, device=cuda_device).to(torch.float8_e4m3fn)
+    scales = torch.zeros(n_pages, device=cuda_device)
+    page_write(x.expand(2, 3, d), t, codes, scales)
+    rows = codes[t.page_ids[:2].long()].float()
+    assert rows.any() and torch.equal(rows, rows[0, 0].expand_as(rows))
+
+
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("norm", ["l2", "rms", "none"])
 def test_write_non_finite_poisons_its_page_only(value, norm, cuda_device):
@@ -220,6 +245,31 @@ def test_write_extreme_magnitudes(cuda_device):
     scales = torch.zeros(n_pages, device=cuda_device)
     page_write(x.cuda(), t, codes, scales, norm="none")
     _check_written(codes, scales, t, lengths, x.double().numpy(), page)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_write_eps_and_weights(dtype, cuda_device):
+    """Rows below and above eps, no eps at all, zero and tiny weights."""
+    from tilemaxsim_b200 import page_write
+    d, page, lengths = 32, 16, [5, 16, 3]
+    x = torch.randn(24, d, generator=_rng(1)).to(dtype)
+    x[3] *= 1e-3
+    t, n_pages = _layout(lengths, page, 2)
+    w = torch.ones(d).to(dtype)
+    w[::3] = 0
+    w[1] = 1e-7
+    for norm, eps, weight in (("l2", 3.0, None), ("l2", 0.0, None), ("rms", 0.0, None), ("rms", 0.5, w),
+                              ("rms", 1e-6, torch.zeros(d).to(dtype)), ("rms", 1e-6, w * 1e-30 if dtype != torch.float16 else w)):
+        codes = torch.zeros(n_pages, page, d, device=cuda_device).to(torch.float8_e4m3fn)
+        scales = torch.zeros(n_pages, device=cuda_device)
+        page_write(x.cuda(), t, codes, scales, norm=norm, eps=eps, weight=None if weight is None else weight.cuda())
+        y = R.normalise(x.double().numpy(), None, None if weight is None else weight.double().numpy(), norm, eps)
+        _check_written(codes, scales, t, lengths, y, page)
+    # a zero row has no direction without an eps: its page is not a number
+    x[7] = 0
+    for norm in ("l2", "rms"):
+        page_write(x.cuda(), t, codes, scales, norm=norm, eps=0.0)
+        assert torch.isnan(scales[t.page_ids[:3].long()]).tolist() == [False, True, False]  # one page a document
 
 
 def test_write_malformed_tables_stay_inside(cuda_device):

@@ -667,11 +667,11 @@ page_write_kernel(const WriteArgs a, int group) {
         const int row = r0 + (mine + i) * step;
         if (i >= held || row >= e.count) break;
         float f = 1.f;
-        odd |= !((usual(tops[i]) || (WEIGHT && tops[i] == 0.f)) && usual(sums[i])) && !(sums[i] == 0.f && tops[i] == 0.f);
+        odd |= !(usual(tops[i]) && usual(sums[i])) && !(sums[i] == 0.f && tops[i] == 0.f);
         if (a.norm != TMS_NORM_NONE) {
           if (a.norm == TMS_NORM_L2) {
             f = sums[i] > 0.f ? rsqrtf(sums[i]) : 1.f;
-            odd |= sums[i] > 0.f && !(f * a.eps < 0.999f);  // at or under eps
+            odd |= sums[i] > 0.f ? !(f * a.eps < 0.999f) : a.eps == 0.f;  // at or under eps; 0 / 0
           } else {
             f = rsqrtf(fmaf(sums[i], per_d, a.eps));
           }
@@ -826,7 +826,7 @@ struct ReadArgs {
 // lane (one 16-byte load), and a thread ROWS rows, whose loads are all in flight before the first
 // store: what bounds it is memory. The output is written past the caches' working set. 3.6M rows of
 // 128 to bf16 take 253 us with two rows and 235 us with four (5.8 TB/s), 182 thousand to fp16 take
-// 12.6 and 14.9 us: four where that makes eight CTAs an SM and more, two below.
+// 12.6 and 14.9 us: four where that makes 32 CTAs an SM and more, two below.
 
 template <typename T>
 __device__ __forceinline__ uint32_t two_as(float x, float y) {
@@ -901,7 +901,7 @@ void launch_read(const ReadArgs& a, const DeviceInfo* dev, cudaStream_t st) {
   int group = 1;  // lanes of a row
   while (group * 16 < a.d) group <<= 1;
   const int64_t rows = 256 / group, most = static_cast<int64_t>(dev->num_sms) * 16;
-  const bool many = a.n_slots >= rows * 4 * dev->num_sms * 8;
+  const bool many = a.n_slots >= rows * 4 * dev->num_sms * 32;
   const int64_t each = rows * (many ? 4 : 2);
   const int64_t blocks = (a.n_slots + each - 1) / each;
   const unsigned grid = static_cast<unsigned>(blocks < most ? blocks : most);

@@ -52,6 +52,10 @@ def _device(*tensors: torch.Tensor) -> torch.device:
     return tensors[0].device
 
 
+def _workspace(nbytes: int, dev: torch.device) -> tuple[torch.Tensor | None, int | None]:
+    return _lib.workspace(nbytes, dev, align=256) if nbytes else (None, None)
+
+
 def _page_size(page_size: int) -> int:
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
@@ -76,7 +80,7 @@ def _tables_call(lengths, doc_ids, src_offsets, pages, page_size, n_tokens, with
         out = PageTables(empty(n_docs + 1, torch.int64), empty(capacity, torch.int32), empty(capacity, torch.int32),
                          empty(n_docs + 1, torch.int64), empty(n_tokens, torch.int64) if with_slots else None)
         ws_bytes = lib.tms_page_tables_workspace_size(n_docs, capacity)
-        ws, ws_ptr = _lib.workspace(ws_bytes, dev, align=256)
+        ws, ws_ptr = _workspace(ws_bytes, dev)
         rc = lib.tms_page_tables(
             _ptr(lengths), lengths.numel(), _ptr(doc_ids), n_docs, _ptr(src_offsets), _ptr(pages), pages.numel(),
             page_size, _ptr(out.page_offsets), _ptr(out.token_offsets), _ptr(out.page_ids), _ptr(out.page_docs),
@@ -134,16 +138,28 @@ def _check_pool(codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int, in
 
 
 def _check_tables(t: PageTables) -> int:
-    if any(x.dim() != 1 or x.dtype != torch.int64 or not x.is_contiguous() for x in (t.page_offsets, t.token_offsets)):
+    offsets, ids, docs, tokens = t.page_offsets, t.page_ids, t.page_docs, t.token_offsets
+    i64, i32 = torch.int64, torch.int32
+    if not (offsets.dtype is i64 and tokens.dtype is i64 and offsets.dim() == 1 and tokens.dim() == 1
+            and offsets.is_contiguous() and tokens.is_contiguous()):
         raise ValueError("page_offsets and token_offsets must be contiguous 1-D int64 tensors")
-    if any(x.dim() != 1 or x.dtype != torch.int32 or not x.is_contiguous() for x in (t.page_ids, t.page_docs)):
+    if not (ids.dtype is i32 and docs.dtype is i32 and ids.dim() == 1 and docs.dim() == 1
+            and ids.is_contiguous() and docs.is_contiguous()):
         raise ValueError("page_ids and page_docs must be contiguous 1-D int32 tensors")
-    if t.page_ids.numel() != t.page_docs.numel():
+    if ids.numel() != docs.numel():
         raise ValueError("page_ids and page_docs must have the same length")
-    n = t.page_offsets.numel() - 1
-    if n < 0 or t.token_offsets.numel() != n + 1:
+    n = offsets.numel() - 1
+    if n < 0 or tokens.numel() != n + 1:
         raise ValueError("page_offsets and token_offsets must have n_docs + 1 entries each")
     return n
+
+
+def _fits(t: torch.Tensor) -> bool:
+    """Whether rows of t can be read 16 bytes at a time as they lie."""
+    if t.data_ptr() % 16:
+        return False
+    each = 16 // t.element_size()  # elements of 16 bytes; a contiguous row has a multiple of them
+    return t.is_contiguous() or (t.stride(-1) == 1 and all(s % each == 0 and s >= 0 for s in t.stride()[:-1]))
 
 
 def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales: torch.Tensor, *,
@@ -180,20 +196,16 @@ def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales:
         raise ValueError("residual must have the shape and dtype of x")
     if weight is not None and (weight.shape != (d,) or weight.dtype != x.dtype):
         raise ValueError(f"weight must be ({d},) {x.dtype}, got {tuple(weight.shape)} {weight.dtype}")
-    rows = 16 // x.element_size()  # elements of 16 bytes
-
-    def fits(t):
-        return t.stride(-1) == 1 and all(s % rows == 0 and s >= 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0
-
     with _lib.on_device(dev):
-        if not fits(x) or (residual is not None and (not fits(residual) or residual.stride() != x.stride())):
+        if not _fits(x) or (residual is not None and (not _fits(residual) or residual.stride() != x.stride())):
             x = x.clone(memory_format=torch.contiguous_format)
             residual = None if residual is None else residual.clone(memory_format=torch.contiguous_format)
         if weight is not None:
             weight = weight.contiguous()
             weight = weight if weight.data_ptr() % 16 == 0 else weight.clone()
         rc = lib.tms_page_write(
-            _ptr(x), _lib.DTYPE_CODE[x.dtype], x.shape[-2], x.stride(0) if padded else 0, x.stride(-2), int(padded),
+            _ptr(x), _lib.DTYPE_CODE[x.dtype], x.shape[-2], x.stride(0) if padded and n_docs > 1 else 0,
+            x.stride(-2) if x.shape[-2] > 1 else d, int(padded),  # a dimension of one may have any stride
             _ptr(residual), _ptr(weight), _NORMS[norm], eps, d, page_size, _ptr(tables.page_offsets),
             _ptr(tables.token_offsets), _ptr(tables.page_ids), _ptr(tables.page_docs), n_docs,
             tables.page_ids.numel(), _ptr(codes), _ptr(scales), n_pages, _lib.stream_handle(dev))
@@ -247,7 +259,7 @@ def paged_maxsim(Qb: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, ta
         out = torch.empty((Bq, n_docs), dtype=torch.float32, device=dev)
         if Bq > 0 and n_docs > 0:
             ws_bytes = lib.tms_paged_workspace_size(Bq, Nq, d, n_docs, page_size, tables.page_ids.numel())
-            ws, ws_ptr = _lib.workspace(ws_bytes, dev, align=256)
+            ws, ws_ptr = _workspace(ws_bytes, dev)
             rc = lib.tms_paged_maxsim(
                 _ptr(Qb), _lib.DTYPE_CODE[Qb.dtype], Bq, Nq, d, _ptr(codes), _ptr(scales), n_pages, page_size,
                 _ptr(tables.page_offsets), _ptr(tables.page_ids), _ptr(tables.page_docs), n_docs,
