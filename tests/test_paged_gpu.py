@@ -248,6 +248,28 @@ def test_write_extreme_magnitudes(cuda_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("amax", [224, 7, 112, 251, 13])
+def test_write_ties_go_to_even(amax, dtype, cuda_device):
+    """Whole numbers as they are: many lie exactly between two codes where the scale is a power of two,
+    and a rounding of the scale away from it where it is not. The codes are those of x / scale in 64 bits."""
+    from tilemaxsim_b200 import page_write
+    d, page, n = 128, 32, 320
+    x = torch.randint(-amax, amax + 1, (n, d), generator=_rng(amax)).to(dtype)
+    x[:, 0] = amax
+    t, n_pages = _layout([n], page, 2)
+    codes = torch.zeros(n_pages, page, d, device=cuda_device).to(torch.float8_e4m3fn)
+    scales = torch.zeros(n_pages, device=cuda_device)
+    page_write(x.cuda(), t, codes, scales, norm="none")
+    scale = float(np.float32(amax / 448))
+    ids = t.page_ids[:n // page].long()
+    assert (scales[ids] == scale).all()
+    v = x.double().numpy() / scale
+    step = 2 * R.half_step(v)
+    want = np.clip(np.round(v / step) * step, -448, 448)  # np.round: ties to even
+    np.testing.assert_array_equal(codes[ids].cpu().double().numpy().reshape(n, d), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_write_eps_and_weights(dtype, cuda_device):
     """Rows below and above eps, no eps at all, zero and tiny weights."""
     from tilemaxsim_b200 import page_write
