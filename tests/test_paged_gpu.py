@@ -269,6 +269,37 @@ def test_write_ties_go_to_even(amax, dtype, cuda_device):
     np.testing.assert_array_equal(codes[ids].cpu().double().numpy().reshape(n, d), want)
 
 
+@pytest.mark.parametrize("amax", [448.0, 1.0, 0.7310585, 3.3333333e-9, 2.9e20])
+def test_write_values_beside_midpoints(amax, cuda_device):
+    """fp32 values at, and up to three steps beside, every midpoint between two codes, the scale's
+    rounding included: one rounding of x / scale, none before it."""
+    from tilemaxsim_b200 import page_write
+    scale = np.float32(np.float64(np.float32(amax)) / 448)
+    codes = np.arange(0x7f, dtype=np.uint8)
+    values = torch.from_numpy(codes).view(torch.float8_e4m3fn).double().numpy()
+    middles = (values[1:] + values[:-1]) / 2
+    near = (middles * np.float64(scale)).astype(np.float32)
+    rows = [near]
+    up, down = near, near
+    for _ in range(3):
+        up, down = np.nextafter(up, np.float32(np.inf)), np.nextafter(down, np.float32(0))
+        rows += [up, down]
+    rows = np.stack(rows + [-r for r in rows])
+    x = np.zeros((16, 128), np.float32)
+    x[:len(rows), :near.size] = rows
+    x[:, 127] = np.float32(amax)
+    t, n_pages = _layout([16], 16, 2)
+    pool = torch.zeros(n_pages, 16, 128, device=cuda_device).to(torch.float8_e4m3fn)
+    scales = torch.zeros(n_pages, device=cuda_device)
+    page_write(torch.from_numpy(x).cuda(), t, pool, scales, norm="none")
+    ids = t.page_ids[:1].long()
+    assert scales[ids].item() == scale
+    v = x.astype(np.float64) / np.float64(scale)  # 2^-53 off: no fp32 quotient is that near a midpoint unless on it
+    step = 2 * R.half_step(v)
+    want = np.clip(np.round(v / step) * step, -448, 448)
+    np.testing.assert_array_equal(pool[ids].cpu().double().numpy().reshape(16, 128), want)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_write_eps_and_weights(dtype, cuda_device):
     """Rows below and above eps, no eps at all, zero and tiny weights."""

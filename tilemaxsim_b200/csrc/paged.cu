@@ -412,7 +412,9 @@ struct Eight {
 // comes within 2^-19 of the page's can set the scale: they (one, as a rule) are summed again in
 // fp64. A code is that of t = h * w * factor / scale: where t * (1 - 2^-20) and t * (1 + 2^-20)
 // round to the same one, fp32 is sure of it; the others (about one of 4,000 groups of eight
-// elements) are done again in fp64, with a division: where nothing is normalised, exact ties are real. Pages that hold a magnitude or a sum of squares outside [1e-30,
+// elements) are done again in fp64, with a division. Where nothing is normalised, added or weighted,
+// ties are common and exact, and one fp32 division with its remainder decides them (5,000 documents:
+// 192 us against 247 with fp64's). Pages that hold a magnitude or a sum of squares outside [1e-30,
 // 1e30], zeros apart, go through fp64 altogether; NaN and infinities are found there.
 //
 // 20,000 documents (3.6M tokens, 128 bf16 values, unit length) take 530 us, 2.7 TB/s: issue slots
@@ -427,6 +429,19 @@ __device__ __forceinline__ bool usual(float v) { return v >= 1e-30f && v <= 1e30
 template <typename T, bool SUM, bool STAGED>
 constexpr int write_threads() { return sizeof(T) == 2 && !SUM && STAGED ? 64 : 128; }
 constexpr int kStageBytes = 24 * 1024;  // most input of a page (x and residual) that is staged
+
+// h / scale to fp32, moved off a midpoint between two codes to the side of the true quotient, where
+// that is not the midpoint itself. Codes are 2^-3 of the leading power of two apart, 2^-9 below 2^-6:
+// there 2^-6 is added to look, which has the same spacing. A midpoint ends in 0x80000.
+__device__ __forceinline__ float off_midpoint(float h, float scale) {
+  const float q = __fdiv_rn(h, scale), m = fabsf(q);
+  const float level = m < 0.015625f ? m + 0.015625f : m;
+  if ((__float_as_uint(level) & 0xfffffu) != 0x80000u) return q;
+  if (m < 0.015625f && level - 0.015625f != m) return q;  // beside a midpoint, lost in the sum
+  const float rest = fmaf(-q, scale, h);  // exact
+  if (rest == 0.f) return q;
+  return __uint_as_float(__float_as_uint(q) + ((rest > 0.f) == (q > 0.f) ? 1u : 0xffffffffu));
+}
 
 struct Entry {    // where a table entry's rows come from
   int64_t at;     // element offset of its first row
@@ -753,7 +768,18 @@ page_write_kernel(const WriteArgs a, int group) {
           word[j >> 2] = e4m3x4(f2_unpack(f2_mul(p0, lo2)), f2_unpack(f2_mul(p1, lo2)));
           other[j >> 2] = e4m3x4(f2_unpack(f2_mul(p0, hi2)), f2_unpack(f2_mul(p1, hi2)));
         }
-        if (!plain || !usual(g) || ((word[0] ^ other[0]) | (word[1] ^ other[1]))) unsure |= 1u << i;
+        if (!plain || !usual(g)) {
+          unsure |= 1u << i;
+        } else if ((word[0] ^ other[0]) | (word[1] ^ other[1])) {
+          if (!SUM && !WEIGHT && a.norm == TMS_NORM_NONE) {  // h is exact, and so is the remainder of h / scale
+#pragma unroll
+            for (int j = 0; j < 8; j += 4)
+              word[j >> 2] = e4m3x4(make_float2(off_midpoint(x.at(j), scale), off_midpoint(x.at(j + 1), scale)),
+                                    make_float2(off_midpoint(x.at(j + 2), scale), off_midpoint(x.at(j + 3), scale)));
+          } else {
+            unsure |= 1u << i;
+          }
+        }
         if (in_row) *reinterpret_cast<uint2*>(out + row * a.d) = make_uint2(word[0], word[1]);
       }
       // Rows that fp32 is not sure of, again.
