@@ -554,6 +554,86 @@ def test_scores_other_stream_and_graph(cuda_device):
     assert torch.equal(a(Q), want.cpu())
 
 
+@pytest.mark.parametrize("n_docs", [30, 2500])
+def test_chain_captured_and_replayed(n_docs, cuda_device):
+    """Tables, writes, scores and reads in one graph: replays follow the lengths and tokens they find."""
+    from tilemaxsim_b200 import GraphedStep, page_read, page_tables, page_write, paged_maxsim
+    d, page, rows = 64, 16, 6
+    bound = n_docs * rows
+    pages = torch.randperm(n_docs, generator=_rng(3)).to(torch.int32).to(cuda_device)
+    codes = torch.zeros(n_docs, page, d, device=cuda_device).to(torch.float8_e4m3fn)
+    scales = torch.zeros(n_docs, device=cuda_device)
+    Q = _queries(3, 32, d, 4, torch.float16)
+
+    def chain(lengths, x):
+        t = page_tables(lengths, page, pages, bound)
+        page_write(x, t, codes, scales)
+        return paged_maxsim(Q, codes, scales, t), page_read(codes, scales, t.slots, torch.float32)
+
+    def example(seed):
+        lengths = torch.randint(0, rows + 1, (n_docs,), generator=_rng(seed))
+        return lengths, torch.randn(n_docs, rows, d, generator=_rng(seed + 1)).half()
+
+    step = GraphedStep(chain, *(v.to(cuda_device) for v in example(1)))
+    for seed in (10, 20, 1):
+        lengths, x = (v.to(cuda_device) for v in example(seed))
+        scores, tokens = step(lengths, x)
+        want_scores, want_tokens = chain(lengths, x)
+        assert torch.equal(scores, want_scores.cpu()) and torch.equal(tokens, want_tokens.cpu())
+        docs = [v.double().numpy() for v in tokens[:int(lengths.sum())].split(lengths.tolist())]
+        _check_scores(want_scores, Q, docs)
+        assert not tokens[int(lengths.sum()):].any()
+
+
+def test_two_streams_at_once(cuda_device):
+    """Calls that overlap on the device share nothing: each kind on one stream against another on the other."""
+    from tilemaxsim_b200 import page_read, paged_maxsim, select_page_tables
+    lengths = torch.randint(0, 300, (400,), generator=_rng(8)).tolist()
+    t, codes, scales, _ = _corpus(lengths, 32, 128, 4)
+    dev_lengths = torch.tensor(lengths, device=cuda_device)
+    pick = torch.randint(0, 400, (300,), generator=_rng(9)).to(cuda_device)
+
+    def rerank(Q):
+        sel = select_page_tables(dev_lengths, 32, t.page_offsets, t.page_ids, pick, 300 * 300)
+        return paged_maxsim(Q, codes, scales, sel), page_read(codes, scales, sel.slots)
+
+    Qs = [_queries(1, 32, 128, 5, torch.bfloat16), _queries(20, 40, 128, 6, torch.float16)]
+    want = [rerank(Q) for Q in Qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in Qs]
+    got = [[], []]
+    for _ in range(20):
+        for s, Q, out in zip(streams, Qs, got):
+            with torch.cuda.stream(s):
+                out.append(rerank(Q))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, w))
+
+
+@pytest.mark.parametrize("page,d", [(128, 256), (16, 128)])
+def test_pool_of_more_than_4_gib(page, d, cuda_device):
+    """Pages whose bytes lie beyond 32-bit offsets, and those that 32 bits would take them for."""
+    from tilemaxsim_b200 import page_read, page_tables, page_write, paged_maxsim
+    wrap = 2 ** 32 // (page * d)
+    n_pages = wrap + 100
+    codes = torch.zeros(n_pages, page, d, dtype=torch.uint8, device=cuda_device).view(torch.float8_e4m3fn)
+    scales = torch.zeros(n_pages, device=cuda_device)
+    lengths = [200, 1, 130, 64]
+    need = sum(-(-n // page) for n in lengths)
+    high = wrap + torch.randperm(100, generator=_rng(1))[:need]
+    x = torch.randn(sum(lengths), d, generator=_rng(2)).half().to(cuda_device)
+    t = page_tables(torch.tensor(lengths).to(cuda_device), page, high.to(torch.int32).to(cuda_device), sum(lengths))
+    page_write(x, t, codes, scales)
+    assert not codes[:100].view(torch.uint8).any() and not scales[:100].any()
+    tokens = page_read(codes, scales, t.slots, torch.float32).cpu().double()
+    y = torch.nn.functional.normalize(x.double().cpu(), dim=-1)
+    most = y.abs().amax()
+    assert ((tokens - y).abs() <= y.abs() * 2.0 ** -4 * 1.001 + most * 2.0 ** -10 / 448 * 1.001).all()
+    Q = _queries(2, 32, d, 3, torch.float16)
+    _check_scores(paged_maxsim(Q, codes, scales, t), Q, [v.numpy() for v in tokens.split(lengths)])
+
+
 @pytest.mark.parametrize("bq", [1, 2, 9])
 def test_scores_bounded_wait_reports_timeout(bq, cuda_device):
     """The loads stay out: every wait runs out after the (short) limit, the kernel returns, the host

@@ -171,8 +171,9 @@ def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales:
 
     x: the tokens of all documents (T, d), document i's at token_offsets[i].., or a padded batch
     (n_docs, L, d) whose document i has its tokens in the first rows (lengths must not exceed L);
-    fp16, bf16 or fp32; residual: same shape and dtype; weight: (d,) of x's dtype. codes and scales are updated in place and
-    returned; pages that the tables do not name keep their content."""
+    fp16, bf16 or fp32; residual: same shape and dtype; weight: (d,) of x's dtype. codes and scales
+    are updated in place and returned; pages that the tables do not name keep their content. A page
+    belongs to one document: of one that the tables name twice the content is undefined."""
     lib = _lib.load()
     if norm not in _NORMS:
         raise ValueError(f"norm must be one of {sorted(_NORMS)}, got {norm!r}")
@@ -183,8 +184,8 @@ def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales:
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     n_pages, page_size, d = _check_pool(codes, scales)
     n_docs = _check_tables(tables)
-    dev = _device(x, codes, scales, tables.page_offsets, tables.page_ids, tables.page_docs,
-                            tables.token_offsets, *(t for t in (residual, weight) if t is not None))
+    dev = _device(x, codes, scales, tables.page_offsets, tables.page_ids, tables.page_docs, tables.token_offsets,
+                  *(t for t in (residual, weight) if t is not None))
     if x.dtype not in _lib.DTYPE_CODE:
         raise TypeError(f"unsupported dtype {x.dtype}; use float16, bfloat16 or float32")
     if x.dim() not in (2, 3) or x.shape[-1] != d:
