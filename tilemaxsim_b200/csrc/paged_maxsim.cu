@@ -54,7 +54,8 @@ constexpr int kJoinBarrier = 2;   // named barrier of the epilogue warps: the st
 constexpr int kTile = 256;        // token columns of a tile
 constexpr int kStages = 6, kSlots = 4;  // at most
 constexpr uint32_t kRow = 128;          // bytes of a row in one K chunk
-constexpr uint32_t kStageBytes = kTile * kRow;  // a stage holds one K chunk of a tile
+// Bytes of a stage, which holds one K chunk of a tile; in pairs, two tokens share a row.
+constexpr uint32_t stage_bytes(bool pair) { return kTile * kRow / (pair ? 2 : 1); }
 constexpr int kQueue = 16;        // documents of an epilogue warp's queue
 constexpr int kQueueStride = 33;  // floats; the odd stride keeps both accesses conflict-free
 constexpr int kMostMt = 4;        // most M tiles of a CTA
@@ -104,12 +105,12 @@ struct SmemLayout {
   uint32_t q, q_bytes, stage, queue, best, head, factor, bars, streams, misc, total;
 };
 
-__host__ __device__ inline SmemLayout smem_layout(int nc, int mt, int terms, int kc, int stages) {
+__host__ __device__ inline SmemLayout smem_layout(int nc, int mt, int terms, int kc, int stages, bool pair) {
   SmemLayout L;
   L.q = 0;
   L.q_bytes = static_cast<uint32_t>(terms * kc * nc * 32) * kRow;  // of one M tile
   L.stage = static_cast<uint32_t>(mt) * L.q_bytes;
-  L.queue = L.stage + static_cast<uint32_t>(stages) * kStageBytes;
+  L.queue = L.stage + static_cast<uint32_t>(stages) * stage_bytes(pair);
   L.best = L.queue + 8u * kQueue * kQueueStride * 4u;
   L.head = L.best + 8u * static_cast<uint32_t>(mt) * 128u;
   L.factor = L.head + 8u * static_cast<uint32_t>(mt) * 128u;
@@ -148,6 +149,25 @@ __device__ __forceinline__ float max_columns(const uint32_t* r) {
       m[i] = max3_nan(m[i], __uint_as_float(r[26 + 2 * i]), __uint_as_float(r[27 + 2 * i]));
   }
   return max3_nan(max3_nan(m[0], m[1], m[2]), max_nan(m[3], m[4]), rest);
+}
+
+// The same of 16 columns in two groups of eight, 16 columns apart.
+__device__ __forceinline__ float max_columns_pair(const uint32_t* r) {
+  const float a = max3_nan(__uint_as_float(r[0]), __uint_as_float(r[1]), __uint_as_float(r[2]));
+  const float b = max3_nan(__uint_as_float(r[3]), __uint_as_float(r[4]), __uint_as_float(r[5]));
+  const float c = max3_nan(__uint_as_float(r[6]), __uint_as_float(r[7]), __uint_as_float(r[16]));
+  const float d = max3_nan(__uint_as_float(r[17]), __uint_as_float(r[18]), __uint_as_float(r[19]));
+  const float e = max3_nan(__uint_as_float(r[20]), __uint_as_float(r[21]), __uint_as_float(r[22]));
+  return max3_nan(max3_nan(a, b, c), max_nan(d, e), __uint_as_float(r[23]));
+}
+// 32 lanes x 16 columns, asynchronous, into r[0..15]; valid after tmem_wait_ld32.
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
 
 // One lane of a converged warp.
@@ -191,6 +211,12 @@ __device__ __forceinline__ void mma_f8_ws(uint32_t d_tmem, uint64_t adesc, uint6
   else if constexpr (KEEP == 1) TMS_MMA_WS("use");
   else TMS_MMA_WS("lastuse");
 #undef TMS_MMA_WS
+}
+// mbar_wait by a converged warp.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, uint64_t timeout_ns,
+                                          uint32_t* err, uint32_t site) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, timeout_ns, err, site));
 }
 // Arrives on `bar` when the MMAs issued so far by the leader are done.
 __device__ __forceinline__ void commit(uint32_t bar, uint32_t leader) {
@@ -333,8 +359,9 @@ __global__ void __launch_bounds__(256) paged_pack_kernel(const PagedArgs a, uint
               factor + static_cast<int64_t>(m) * 128);
 }
 
-// NC: chunks of an M tile (1, 2 or 4); U: rows of a box (16 or 32).
-template <int NC, int U>
+// NC: chunks of an M tile (1, 2 or 4); U: tokens of a box (16 or 32); PAIR: d = 64, and two tokens to a
+// row of 128 bytes, in memory and in a stage.
+template <int NC, int U, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_constant__ PagedArgs a) {
   constexpr int kStreams = 8 / NC;
@@ -345,7 +372,9 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
   constexpr uint32_t kAllWarp = 0xffffffffu;
   static_assert(kCols == 2 * W && 32 % kUnits == 0 && 2 * kUnits <= kQueue, "two warps a lane quarter");
   extern __shared__ __align__(1024) uint8_t smem[];
-  const SmemLayout L = smem_layout(NC, a.mt, a.terms, a.kc, a.stages);
+  constexpr int kBoxRows = PAIR ? U / 2 : U;
+  constexpr uint32_t kStageBytes = stage_bytes(PAIR);
+  const SmemLayout L = smem_layout(NC, a.mt, a.terms, a.kc, a.stages, PAIR);
   const int warp = uniform(threadIdx.x >> 5), lane = lane_id();
   const int group = blockIdx.x % a.groups, range = blockIdx.x / a.groups;
   const int m_first = group * a.mt;
@@ -488,22 +517,28 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       ids[i] = page_of(unit + kAhead * kUnits);
       const bool load = id >= 0 && id < a.n_pages;
       const uint32_t mask = __ballot_sync(kAllWarp, load), boxes = __popc(mask);
-      const int32_t y = static_cast<int32_t>(id << a.page_shift) + (unit & half_mask) * U;
+      const int32_t y = static_cast<int32_t>(id << (a.page_shift - PAIR)) + (unit & half_mask) * kBoxRows;
+      int32_t rows[kTile / U];  // of all boxes, before the first load: a shuffle between loads holds them up
+#pragma unroll
+      for (int b = 0; b < kTile / U; ++b) rows[b] = __shfl_sync(kAllWarp, y, b);
       for (int c = 0; c < a.kc; ++c) {
-        ok = mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, a.timeout_ns, a.err, 41);
-        ok = __all_sync(kAllWarp, ok);
+        ok = warp_wait(empty_bar(s), ph ^ 1u, abort_flag, a.timeout_ns, a.err, 41);
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(full_bar(s), boxes * static_cast<uint32_t>(U * kRow));
+        if (lane == 0) mbar_arrive_expect_tx(full_bar(s), boxes * static_cast<uint32_t>(kBoxRows * kRow));
         armed |= 1u << s;
         armed_par = (armed_par & ~(1u << s)) | (ph << s);
         __syncwarp();
+        if (boxes == kTile / U) {
 #pragma unroll
-        for (int b = 0; b < kTile / U; ++b) {
-          const int yb = __shfl_sync(kAllWarp, y, b);
+          for (int b = 0; b < kTile / U; ++b)
+            box_load(base + L.stage + static_cast<uint32_t>(s) * kStageBytes + b * kBoxRows * kRow, &codes_map, full_bar(s),
+                     c * 128, rows[b], policy, leader);
+        } else
+#pragma unroll
+        for (int b = 0; b < kTile / U; ++b)
           if (mask >> b & 1u)
-            box_load(base + L.stage + static_cast<uint32_t>(s) * kStageBytes + b * U * kRow, &codes_map, full_bar(s),
-                     c * 128, yb, policy, leader);
-        }
+            box_load(base + L.stage + static_cast<uint32_t>(s) * kStageBytes + b * kBoxRows * kRow, &codes_map, full_bar(s),
+                     c * 128, rows[b], policy, leader);
         if (++s == a.stages) { s = 0; ph ^= 1u; }
       }
      }
@@ -516,9 +551,12 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
     const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(*tmem_slot)));
     if (warp == 1) {
       // ---------------------------------------------------------------- MMA issue
-      constexpr uint32_t idesc = make_idesc(32 * NC, kTile, 0);  // e4m3 operands, fp32 accumulator
+      constexpr uint32_t idesc = make_idesc(32 * NC, PAIR ? kTile / 2 : kTile, 0);  // e4m3 operands, fp32 accumulator
       const uint32_t leader = elect_one();
-      const uint64_t a0 = sw128_kmajor_desc(base + L.q), b0 = sw128_kmajor_desc(base + L.stage);
+      const uint64_t desc0 = sw128_kmajor_desc(0);
+      auto desc = [&](uint32_t lo) { return desc0 & ~0xffffffffull | lo; };  // steps stay in the low word
+      const uint32_t a0 = static_cast<uint32_t>(sw128_kmajor_desc(base + L.q));
+      const uint32_t b0 = static_cast<uint32_t>(sw128_kmajor_desc(base + L.stage));
       const uint32_t term_step = static_cast<uint32_t>(a.kc * 32 * NC) * kRow >> 4;  // in descriptor units
       const int terms = a.terms, kc = a.kc, stages = a.stages;
       const int last_steps = (a.d - (kc - 1) * 128 + 31) / 32;  // 32-element steps of the last chunk
@@ -528,30 +566,44 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       if (a.packed) ok = __all_sync(kAllWarp, mbar_wait(query_bar, 0, abort_flag, a.timeout_ns, a.err, 48));
       for (int t = 0; ok && t < n_tiles; ++t) {
         for (int m = 0; m < mt; ++m) {
-          ok = __all_sync(kAllWarp, mbar_wait(acce_bar(slot), acc_ph, abort_flag, a.timeout_ns, a.err, 44));
+          ok = warp_wait(acce_bar(slot), acc_ph, abort_flag, a.timeout_ns, a.err, 44);
           if (!ok) break;
           tc_fence_after();
-          uint32_t acc = 0;
           for (int c = 0; c < kc; ++c) {  // kc > 1 comes with one M tile
             if (m == 0) {
-              ok = __all_sync(kAllWarp, mbar_wait(full_bar(s), ph, abort_flag, a.timeout_ns, a.err, 43));
+              ok = warp_wait(full_bar(s), ph, abort_flag, a.timeout_ns, a.err, 43);
               if (!ok) break;
               tc_fence_after();
             }
             const int steps = c == kc - 1 ? last_steps : 4;
-            uint64_t ad = a0 + static_cast<uint32_t>(m * L.q_bytes + c * 32 * NC * kRow) / 16;
-            uint64_t bd = b0 + static_cast<uint32_t>(s) * (kStageBytes / 16);
-            for (int k = 0; k < steps; ++k, ad += 2, bd += 2) {
+            const uint32_t a_lo = a0 + static_cast<uint32_t>(m * L.q_bytes + c * 32 * NC * kRow) / 16;
+            const uint32_t b_lo = b0 + static_cast<uint32_t>(s) * (kStageBytes / 16);
+            const uint32_t to = tmem + slot * kCols;
+            auto step = [&](uint32_t to, uint32_t at, uint32_t bt, uint32_t acc) {  // 32 elements of K
               if constexpr (NC == 4) {
-                mma_f8(tmem + slot * kCols, ad, bd, idesc, acc, leader);
-                mma_f8(tmem + slot * kCols, ad + term_step, bd, idesc, 1, leader);
-                if (terms == 3) mma_f8(tmem + slot * kCols, ad + 2 * term_step, bd, idesc, 1, leader);
+                mma_f8(to, desc(at), desc(bt), idesc, acc, leader);
+                mma_f8(to, desc(at + term_step), desc(bt), idesc, 1, leader);
+                if (terms == 3) mma_f8(to, desc(at + 2 * term_step), desc(bt), idesc, 1, leader);
               } else {
-                mma_f8_ws<0>(tmem + slot * kCols, ad, bd, idesc, acc, leader);
-                if (terms == 3) mma_f8_ws<1>(tmem + slot * kCols, ad + term_step, bd, idesc, 1, leader);
-                mma_f8_ws<2>(tmem + slot * kCols, ad + (terms == 3 ? 2 * term_step : term_step), bd, idesc, 1, leader);
+                mma_f8_ws<0>(to, desc(at), desc(bt), idesc, acc, leader);
+                if (terms == 3) {
+                  mma_f8_ws<1>(to, desc(at + term_step), desc(bt), idesc, 1, leader);
+                  mma_f8_ws<2>(to, desc(at + 2 * term_step), desc(bt), idesc, 1, leader);
+                } else {
+                  mma_f8_ws<2>(to, desc(at + term_step), desc(bt), idesc, 1, leader);
+                }
               }
-              acc = 1;
+            };
+            // The issuing warp's own instructions count: one warp alone takes several clocks for each.
+            if constexpr (PAIR) {
+              // first the rows' first tokens, then their second ones, 64 bytes on, into columns of their own
+#pragma unroll
+              for (int k = 0; k < 4; ++k) step(to + (k >> 1) * W, a_lo + 2 * (k & 1), b_lo + 2 * k, k & 1);
+            } else if (steps == 4) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) step(to, a_lo + 2 * k, b_lo + 2 * k, k > 0 || c > 0);
+            } else {
+              for (int k = 0; k < steps; ++k) step(to, a_lo + 2 * k, b_lo + 2 * k, k > 0 || c > 0);
             }
             if (m == mt - 1) {
               commit(empty_bar(s), leader);
@@ -643,10 +695,19 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
         bool still_open = open;
         for (int m = 0; m < mt; ++m) {
           float best = bests[m * 32];
-          ok = __all_sync(kAllWarp, mbar_wait(accf_bar(slot), acc_ph, abort_flag, a.timeout_ns, a.err, 46));
+          ok = warp_wait(accf_bar(slot), acc_ph, abort_flag, a.timeout_ns, a.err, 46);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t at = tmem + slot * kCols + half * W + (static_cast<uint32_t>(quarter * 32) << 16);
+          // In pairs, a stream's first tokens of rows lie in one half of the columns, the second ones in the other.
+          const uint32_t at = tmem + slot * kCols + half * (PAIR ? W / 2 : W) + (static_cast<uint32_t>(quarter * 32) << 16);
+          auto load = [&](int b, uint32_t(&r)[32]) {  // 32 tokens' columns
+            if constexpr (PAIR) {
+              tmem_ld16_async(at + 16 * b, r);
+              tmem_ld16_async(at + W + 16 * b, r + 16);
+            } else {
+              tmem_ld32_async(at + 32 * b, r);
+            }
+          };
           still_open = open;
           auto one = [&](int i, float v) {  // box i of the tile is done
             if (!(scales[i] < 0.f)) best = max_nan(best, v * scales[i]);
@@ -663,14 +724,14 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
             }
           };
           uint32_t ra[32], rb[32];
-          tmem_ld32_async(at, ra);
+          load(0, ra);
 #pragma unroll
           for (int b = 0; b < W / 32; ++b) {
             uint32_t(&cur)[32] = (b & 1) ? rb : ra;
             uint32_t(&nxt)[32] = (b & 1) ? ra : rb;
             tmem_wait_ld32(cur);
             if (b + 1 < W / 32) {
-              tmem_ld32_async(at + 32 * (b + 1), nxt);
+              load(b + 1, nxt);
             } else {  // the accumulator goes back before its last columns are reduced
               tc_fence_before();
               __syncwarp();
@@ -681,7 +742,8 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
               if (plain) best = max_nan(best, v * scales[b]);
               else one(b, v);
             } else {
-              const float v = max_columns<16>(cur), w = max_columns<16>(cur + 16);
+              const float v = PAIR ? max_columns_pair(cur) : max_columns<16>(cur);
+              const float w = PAIR ? max_columns_pair(cur + 8) : max_columns<16>(cur + 16);
               if (plain) {
                 best = max3_nan(best, v * scales[2 * b], w * scales[2 * b + 1]);
               } else {
@@ -803,10 +865,10 @@ int blocks_for(int64_t work, const DeviceInfo* dev) {
   return static_cast<int>(b < 1 ? 1 : b > most ? most : b);
 }
 
-template <int NC, int U>
+template <int NC, int U, bool PAIR>
 int launch(const CUtensorMap& map, const PagedArgs& a, cudaStream_t st) {
-  auto kern = paged_mma_kernel<NC, U>;
-  const uint32_t smem = smem_layout(NC, a.mt, a.terms, a.kc, a.stages).total;
+  auto kern = paged_mma_kernel<NC, U, PAIR>;
+  const uint32_t smem = smem_layout(NC, a.mt, a.terms, a.kc, a.stages, PAIR).total;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess)
     return TMS_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
@@ -820,6 +882,13 @@ int launch(const CUtensorMap& map, const PagedArgs& a, cudaStream_t st) {
   cfg.attrs = &early;
   cfg.numAttrs = a.packed ? 1 : 0;  // the packing kernel is the launch before
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, map, a));
+}
+
+template <int U, bool PAIR>
+int launch_chunks(int nc, const CUtensorMap& map, const PagedArgs& a, cudaStream_t st) {
+  return nc == 1   ? launch<1, U, PAIR>(map, a, st)
+         : nc == 2 ? launch<2, U, PAIR>(map, a, st)
+                   : launch<4, U, PAIR>(map, a, st);
 }
 
 // Workspace: the chunks' scores of queries of more than 32 rows, then the packed query tiles and
@@ -922,15 +991,16 @@ extern "C" int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, i
   a.debug_flags = debug_flags();
 
   const int nc = a.n_chunks < 3 ? a.n_chunks : 4;
+  const bool pair = d == 64;  // half the rows for the TMA to bring
   const uint32_t room = static_cast<uint32_t>(dev->max_smem_optin);
   // As many M tiles a CTA as leave two stages: each tile of tokens is then loaded and held for all
   // of them. With two K chunks a tile's stages pass one by one, so there is one M tile.
   a.mt = a.kc > 1 ? 1 : a.n_mtiles < kMostMt ? a.n_mtiles : kMostMt;
-  while (a.mt > 1 && smem_layout(nc, a.mt, a.terms, a.kc, 2).total > room) --a.mt;
+  while (a.mt > 1 && smem_layout(nc, a.mt, a.terms, a.kc, 2, pair).total > room) --a.mt;
   a.groups = (a.n_mtiles + a.mt - 1) / a.mt;
   a.mt = (a.n_mtiles + a.groups - 1) / a.groups;
   a.stages = 2;
-  while (a.stages < kStages && smem_layout(nc, a.mt, a.terms, a.kc, a.stages + 1).total <= room) ++a.stages;
+  while (a.stages < kStages && smem_layout(nc, a.mt, a.terms, a.kc, a.stages + 1, pair).total <= room) ++a.stages;
   int64_t ranges = dev->num_sms / a.groups;
   if (ranges > page_capacity) ranges = page_capacity;
   a.ranges = static_cast<int>(ranges < 1 ? 1 : ranges);
@@ -949,12 +1019,13 @@ extern "C" int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, i
     a.packed_factor = factor;
   }
   CUtensorMap map;
-  int rc = encode_tmap_2d(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, static_cast<uint64_t>(d),
-                          static_cast<uint64_t>(n_pages * page_size), static_cast<uint64_t>(d), 128,
-                          static_cast<uint32_t>(U));
+  const int64_t row = pair ? 2 * d : d, rows = n_pages * page_size / (pair ? 2 : 1);
+  int rc = encode_tmap_2d(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, static_cast<uint64_t>(row),
+                          static_cast<uint64_t>(rows), static_cast<uint64_t>(row), 128,
+                          static_cast<uint32_t>(pair ? U / 2 : U));
   if (rc != TMS_OK) return rc;
-  if (U == 16) rc = nc == 1 ? launch<1, 16>(map, a, st) : nc == 2 ? launch<2, 16>(map, a, st) : launch<4, 16>(map, a, st);
-  else rc = nc == 1 ? launch<1, 32>(map, a, st) : nc == 2 ? launch<2, 32>(map, a, st) : launch<4, 32>(map, a, st);
+  if (U == 16) rc = pair ? launch_chunks<16, true>(nc, map, a, st) : launch_chunks<16, false>(nc, map, a, st);
+  else rc = pair ? launch_chunks<32, true>(nc, map, a, st) : launch_chunks<32, false>(nc, map, a, st);
   if (rc != TMS_OK) return rc;
   if (a.parts) {
     paged_join_kernel<<<static_cast<unsigned>((static_cast<int64_t>(a.ranges) * a.n_chunks + 7) / 8), 256, 0, st>>>(a);
