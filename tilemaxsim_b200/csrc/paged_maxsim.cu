@@ -37,6 +37,8 @@
 // 32 rows), warp 1 owns TMEM and issues the MMAs, warps 2-9 are the epilogue. A document that ends
 // puts its 32 row maxima into a queue in shared memory; up to sixteen documents are summed at a time
 // (two lanes each), which takes the 5-step shuffle sum per document out of the loop.
+#include <type_traits>
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -566,11 +568,16 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
       if (a.packed) ok = __all_sync(kAllWarp, mbar_wait(query_bar, 0, abort_flag, a.timeout_ns, a.err, 48));
       for (int t = 0; ok && t < n_tiles; ++t) {
         for (int m = 0; m < mt; ++m) {
-          ok = warp_wait(acce_bar(slot), acc_ph, abort_flag, a.timeout_ns, a.err, 44);
-          if (!ok) break;
+          // An accumulator and the tile's first stage, looked at together.
+          const bool both = mbar_try_wait(acce_bar(slot), acc_ph) & (m > 0 || mbar_try_wait(full_bar(s), ph));
+          if (!__all_sync(kAllWarp, both)) {
+            ok = warp_wait(acce_bar(slot), acc_ph, abort_flag, a.timeout_ns, a.err, 44);
+            if (ok && m == 0) ok = warp_wait(full_bar(s), ph, abort_flag, a.timeout_ns, a.err, 43);
+            if (!ok) break;
+          }
           tc_fence_after();
           for (int c = 0; c < kc; ++c) {  // kc > 1 comes with one M tile
-            if (m == 0) {
+            if (c > 0) {
               ok = warp_wait(full_bar(s), ph, abort_flag, a.timeout_ns, a.err, 43);
               if (!ok) break;
               tc_fence_after();
@@ -579,32 +586,32 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
             const uint32_t a_lo = a0 + static_cast<uint32_t>(m * L.q_bytes + c * 32 * NC * kRow) / 16;
             const uint32_t b_lo = b0 + static_cast<uint32_t>(s) * (kStageBytes / 16);
             const uint32_t to = tmem + slot * kCols;
-            auto step = [&](uint32_t to, uint32_t at, uint32_t bt, uint32_t acc) {  // 32 elements of K
+            auto step = [&](auto three, uint32_t to, uint32_t at, uint32_t bt, uint32_t acc) {  // 32 elements of K
               if constexpr (NC == 4) {
                 mma_f8(to, desc(at), desc(bt), idesc, acc, leader);
                 mma_f8(to, desc(at + term_step), desc(bt), idesc, 1, leader);
-                if (terms == 3) mma_f8(to, desc(at + 2 * term_step), desc(bt), idesc, 1, leader);
+                if constexpr (three.value) mma_f8(to, desc(at + 2 * term_step), desc(bt), idesc, 1, leader);
               } else {
                 mma_f8_ws<0>(to, desc(at), desc(bt), idesc, acc, leader);
-                if (terms == 3) {
-                  mma_f8_ws<1>(to, desc(at + term_step), desc(bt), idesc, 1, leader);
-                  mma_f8_ws<2>(to, desc(at + 2 * term_step), desc(bt), idesc, 1, leader);
-                } else {
-                  mma_f8_ws<2>(to, desc(at + term_step), desc(bt), idesc, 1, leader);
-                }
+                if constexpr (three.value) mma_f8_ws<1>(to, desc(at + term_step), desc(bt), idesc, 1, leader);
+                mma_f8_ws<2>(to, desc(at + (three.value ? 2 : 1) * term_step), desc(bt), idesc, 1, leader);
               }
             };
             // The issuing warp's own instructions count: one warp alone takes several clocks for each.
-            if constexpr (PAIR) {
-              // first the rows' first tokens, then their second ones, 64 bytes on, into columns of their own
+            auto all_steps = [&](auto three) {
+              if constexpr (PAIR) {
+                // first the rows' first tokens, then their second ones, 64 bytes on, into columns of their own
 #pragma unroll
-              for (int k = 0; k < 4; ++k) step(to + (k >> 1) * W, a_lo + 2 * (k & 1), b_lo + 2 * k, k & 1);
-            } else if (steps == 4) {
+                for (int k = 0; k < 4; ++k) step(three, to + (k >> 1) * W, a_lo + 2 * (k & 1), b_lo + 2 * k, k & 1);
+              } else if (steps == 4) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) step(to, a_lo + 2 * k, b_lo + 2 * k, k > 0 || c > 0);
-            } else {
-              for (int k = 0; k < steps; ++k) step(to, a_lo + 2 * k, b_lo + 2 * k, k > 0 || c > 0);
-            }
+                for (int k = 0; k < 4; ++k) step(three, to, a_lo + 2 * k, b_lo + 2 * k, k > 0 || c > 0);
+              } else {
+                for (int k = 0; k < steps; ++k) step(three, to, a_lo + 2 * k, b_lo + 2 * k, k > 0 || c > 0);
+              }
+            };
+            if (terms == 3) all_steps(std::true_type());
+            else all_steps(std::false_type());
             if (m == mt - 1) {
               commit(empty_bar(s), leader);
               if (++s == stages) { s = 0; ph ^= 1u; }
