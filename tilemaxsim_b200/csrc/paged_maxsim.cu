@@ -657,26 +657,33 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
         __syncwarp();
         queued = 0;
       };
-      // What the epilogue needs of 32 boxes, a lane for each, fetched 32 boxes ahead: the page's
-      // scale (-1: no page there) and the document that ends with the box (-1: none does).
+      // What the epilogue needs of 32 boxes, a lane for each: the page's scale (-1: no page there) and
+      // the document that ends with the box (-1: none does). Table entries are loaded 64 boxes ahead and
+      // looked at 32 boxes ahead, when the scale is loaded: no load is waited for where it is issued.
       float cur_scale = 0.f, next_scale = 0.f;
       int cur_ends = -1, next_ends = -1;
+      int entry_id = -1, entry_doc = -1, entry_after = -1;  // page, document, the next entry's document
       uint32_t end_mask = 0;  // a bit for each of the 32 boxes with which a document ends
       uint32_t odd_mask = 0;  // and for each that is not a plain page inside a document
-      auto fetch = [&](int u0) {
+      auto entries = [&](int u0) {
         const int u = u0 + lane;
-        next_scale = -1.f;
-        next_ends = -1;
+        entry_id = entry_doc = entry_after = -1;
         if (u < my_units) {
           const int v = my_first + (u >> a.unit_shift);
-          const int64_t id = __ldg(a.page_ids + v);
-          const int doc = __ldg(a.page_docs + v);
-          if (id >= 0 && id < a.n_pages) next_scale = __ldg(a.scales + id);
-          if ((u & half_mask) == half_mask && doc >= 0 && doc < a.n_docs &&
-              (v + 1 >= cta_end || __ldg(a.page_docs + v + 1) != doc))
-            next_ends = doc;
+          entry_id = __ldg(a.page_ids + v);
+          if ((u & half_mask) == half_mask) {
+            entry_doc = __ldg(a.page_docs + v);
+            if (v + 1 < cta_end) entry_after = __ldg(a.page_docs + v + 1);
+          }
         }
       };
+      auto fetch = [&](int u0) {
+        next_scale = -1.f;
+        if (entry_id >= 0 && entry_id < a.n_pages) next_scale = __ldg(a.scales + entry_id);
+        next_ends = entry_doc >= 0 && entry_doc < a.n_docs && entry_after != entry_doc ? entry_doc : -1;
+        entries(u0 + 32);
+      };
+      entries(0);
       fetch(0);
       write_empty();
       for (int m = 0; m < mt; ++m) bests[m * 32] = kNegInf;
@@ -698,7 +705,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) scales[i] = __shfl_sync(kAllWarp, cur_scale, (unit0 + i) & 31);
         const uint32_t ends_here = end_mask >> (unit0 & 31);
-        const bool plain = (odd_mask >> (unit0 & 31) & ((1u << kUnits) - 1u)) == 0;
+        const uint32_t odd_here = odd_mask >> (unit0 & 31);
         bool still_open = open;
         for (int m = 0; m < mt; ++m) {
           float best = bests[m * 32];
@@ -746,12 +753,12 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
             }
             if constexpr (U == 32) {
               const float v = max_columns<32>(cur);
-              if (plain) best = max_nan(best, v * scales[b]);
+              if (!(odd_here >> b & 1u)) best = max_nan(best, v * scales[b]);
               else one(b, v);
             } else {
               const float v = PAIR ? max_columns_pair(cur) : max_columns<16>(cur);
               const float w = PAIR ? max_columns_pair(cur + 8) : max_columns<16>(cur + 16);
-              if (plain) {
+              if (!(odd_here >> 2 * b & 3u)) {
                 best = max3_nan(best, v * scales[2 * b], w * scales[2 * b + 1]);
               } else {
                 one(2 * b, v);
