@@ -417,7 +417,7 @@ struct Eight {
 // 192 us against 247 with fp64's). Pages that hold a magnitude or a sum of squares outside [1e-30,
 // 1e30], zeros apart, go through fp64 altogether; NaN and infinities are found there.
 //
-// 20,000 documents (3.6M tokens, 128 bf16 values, unit length) take 530 us, 2.7 TB/s: issue slots
+// 20,000 documents (3.6M tokens, 128 bf16 values, unit length) take 540 us, 2.6 TB/s: issue slots
 // (64% busy), not memory, bound it. Rows held in registers took 770 us (few warps fit), all sums in
 // fp64 600-820, sixteen elements a lane 546, fp64 roots for the rows that set the scale 830.
 __device__ __forceinline__ double max_keep_nan(double x, double y) { return y <= x || x != x ? x : y; }

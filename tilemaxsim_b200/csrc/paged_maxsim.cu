@@ -25,13 +25,19 @@
 // what a document has in several ranges is joined by a kernel of its own. No atomics, and the sums
 // run in one order: results do not depend on the launch.
 //
+// For one or two chunks, tokens of d = 64 lie two to a row of 128 bytes, in memory as in a stage, which
+// halves the rows that the TMA brings and the stage's bytes: the MMAs take N = 128 rows twice, their first
+// 64 bytes and their second, into the two halves of the columns.
+//
 // What bounds it. One query over 100k documents (18.2M tokens, 2.53 GB of pages): memory, 405 us, 6.2
-// TB/s. 64 queries over 4,000 documents: the tensor cores (87% of their cycles), 245 us, 1,560 TFLOP/s
-// of the query's own products, which the two terms double. 5 queries of 77 rows at d = 256 in fp16
-// (three terms): the tensor cores (92%), 206 us. Pages of 16 rows, or narrow ones, at one to four
-// chunks: the TMA's boxes, about 65 clocks each and 2 a row whatever it holds (d = 64, pages of 16, 5.1M
-// tokens: 146 us); copying them by cp.async took 228 us, the proxy fences waiting for the copies.
-// Under a power cap that lowers the clocks these grow by about a tenth.
+// TB/s. 64 queries over 4,000 documents: the tensor cores, 251 us, 1,520 TFLOP/s of the query's own
+// products, which the two terms double; after a second of it the power cap, 285 us. 5 queries of 77 rows
+// at d = 256 in fp16 (three terms): the tensor cores, 222 us, 240 under the cap. Few chunks of narrow
+// tokens: the instructions that a warp's own loop takes for a tile, where each waits for the one before.
+// 18.2M tokens of d = 64: 260 us, the MMA warp (397 us with loops and 64-bit descriptors around its 8
+// MMAs and one wait after the other). d = 64, pages of 16, 5.1M tokens, 3 queries: 111 us, the epilogue
+// and the 16 boxes a tile (139 us at first). Copying the pages by cp.async in place of the TMA: 154 us with four
+// warps, 181-228 with two.
 //
 // Warp roles (320 threads, one CTA an SM): warp 0 loads pages by TMA (a lane for each box of up to
 // 32 rows), warp 1 owns TMEM and issues the MMAs, warps 2-9 are the epilogue. A document that ends
@@ -530,17 +536,18 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
         armed |= 1u << s;
         armed_par = (armed_par & ~(1u << s)) | (ph << s);
         __syncwarp();
-        if (boxes == kTile / U) {
+        auto load_box = [&](int b) {
+          box_load(base + L.stage + static_cast<uint32_t>(s) * kStageBytes + b * kBoxRows * kRow, &codes_map,
+                   full_bar(s), c * 128, rows[b], policy, leader);
+        };
+        if (boxes == kTile / U) {  // without a branch for each (137 against 132 us with sixteen)
+#pragma unroll
+          for (int b = 0; b < kTile / U; ++b) load_box(b);
+        } else {
 #pragma unroll
           for (int b = 0; b < kTile / U; ++b)
-            box_load(base + L.stage + static_cast<uint32_t>(s) * kStageBytes + b * kBoxRows * kRow, &codes_map, full_bar(s),
-                     c * 128, rows[b], policy, leader);
-        } else
-#pragma unroll
-        for (int b = 0; b < kTile / U; ++b)
-          if (mask >> b & 1u)
-            box_load(base + L.stage + static_cast<uint32_t>(s) * kStageBytes + b * kBoxRows * kRow, &codes_map, full_bar(s),
-                     c * 128, rows[b], policy, leader);
+            if (mask >> b & 1u) load_box(b);
+        }
         if (++s == a.stages) { s = 0; ph ^= 1u; }
       }
      }
@@ -898,13 +905,6 @@ int launch(const CUtensorMap& map, const PagedArgs& a, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, map, a));
 }
 
-template <int U, bool PAIR>
-int launch_chunks(int nc, const CUtensorMap& map, const PagedArgs& a, cudaStream_t st) {
-  return nc == 1   ? launch<1, U, PAIR>(map, a, st)
-         : nc == 2 ? launch<2, U, PAIR>(map, a, st)
-                   : launch<4, U, PAIR>(map, a, st);
-}
-
 // Workspace: the chunks' scores of queries of more than 32 rows, then the packed query tiles and
 // their factors when there are more than two chunks, then the parts of documents cut by ranges.
 struct Workspace {
@@ -1005,7 +1005,10 @@ extern "C" int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, i
   a.debug_flags = debug_flags();
 
   const int nc = a.n_chunks < 3 ? a.n_chunks : 4;
-  const bool pair = d == 64;  // half the rows for the TMA to bring
+  // Two tokens of d = 64 to a row, for one or two chunks: 18.2M tokens 260 us against 328 (pages of 16 rows
+  // 278 against 388), two chunks over 5.1M 96 against 114. With four, the epilogue's twice as many loads
+  // cost more than the TMA gains: 114 against 111, 64 queries 192 against 189.
+  const bool pair = d == 64 && nc < 4;
   const uint32_t room = static_cast<uint32_t>(dev->max_smem_optin);
   // As many M tiles a CTA as leave two stages: each tile of tokens is then loaded and held for all
   // of them. With two K chunks a tile's stages pass one by one, so there is one M tile.
@@ -1038,8 +1041,15 @@ extern "C" int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, i
                           static_cast<uint64_t>(rows), static_cast<uint64_t>(row), 128,
                           static_cast<uint32_t>(pair ? U / 2 : U));
   if (rc != TMS_OK) return rc;
-  if (U == 16) rc = pair ? launch_chunks<16, true>(nc, map, a, st) : launch_chunks<16, false>(nc, map, a, st);
-  else rc = pair ? launch_chunks<32, true>(nc, map, a, st) : launch_chunks<32, false>(nc, map, a, st);
+  if (U == 16) {
+    rc = nc == 4   ? launch<4, 16, false>(map, a, st)
+         : nc == 2 ? (pair ? launch<2, 16, true>(map, a, st) : launch<2, 16, false>(map, a, st))
+                   : (pair ? launch<1, 16, true>(map, a, st) : launch<1, 16, false>(map, a, st));
+  } else {
+    rc = nc == 4   ? launch<4, 32, false>(map, a, st)
+         : nc == 2 ? (pair ? launch<2, 32, true>(map, a, st) : launch<2, 32, false>(map, a, st))
+                   : (pair ? launch<1, 32, true>(map, a, st) : launch<1, 32, false>(map, a, st));
+  }
   if (rc != TMS_OK) return rc;
   if (a.parts) {
     paged_join_kernel<<<static_cast<unsigned>((static_cast<int64_t>(a.ranges) * a.n_chunks + 7) / 8), 256, 0, st>>>(a);
