@@ -414,12 +414,14 @@ struct Eight {
 // round to the same one, fp32 is sure of it; the others (about one of 4,000 groups of eight
 // elements) are done again in fp64, with a division. Where nothing is normalised, added or weighted,
 // ties are common and exact, and one fp32 division with its remainder decides them (5,000 documents:
-// 192 us against 247 with fp64's). Pages that hold a magnitude or a sum of squares outside [1e-30,
+// 196 us against 247 with fp64's). Pages that hold a magnitude or a sum of squares outside [1e-30,
 // 1e30], zeros apart, go through fp64 altogether; NaN and infinities are found there.
 //
-// 20,000 documents (3.6M tokens, 128 bf16 values, unit length) take 540 us, 2.6 TB/s: issue slots
-// (64% busy), not memory, bound it. Rows held in registers took 770 us (few warps fit), all sums in
-// fp64 600-820, sixteen elements a lane 546, fp64 roots for the rows that set the scale 830.
+// 20,000 documents (3.6M tokens, 128 bf16 values, unit length) take 456 us, 3.1 TB/s: issue slots (62%
+// busy), not memory, bound it, which is why the width is a constant of the kernel where it is 128 (D).
+// Without that they take 546 us, and 1,600 pages with a residual 17 us against 14.9; the page size as
+// a constant too would give 2% more. Before, rows held in registers took 770 us (few warps fit), all
+// sums in fp64 600-820, sixteen elements a lane 546, fp64 roots for the rows that set the scale 830.
 __device__ __forceinline__ double max_keep_nan(double x, double y) { return y <= x || x != x ? x : y; }
 __device__ __forceinline__ bool usual(float v) { return v >= 1e-30f && v <= 1e30f; }
 
@@ -428,6 +430,7 @@ __device__ __forceinline__ bool usual(float v) { return v >= 1e-30f && v <= 1e30
 // where pages are not staged.
 template <typename T, bool SUM, bool STAGED>
 constexpr int write_threads() { return sizeof(T) == 2 && !SUM && STAGED ? 64 : 128; }
+constexpr int kStaticBytes = 2048;       // a CTA's other shared memory, at most
 constexpr int kStageBytes = 24 * 1024;  // most input of a page (x and residual) that is staged
 
 // h / scale to fp32, moved off a midpoint between two codes to the side of the true quotient, where
@@ -450,11 +453,11 @@ struct Entry {    // where a table entry's rows come from
   int count;      // 0: the entry is skipped
 };
 
-template <typename T, bool SUM, bool WEIGHT, bool STAGED>
+template <typename T, bool SUM, bool WEIGHT, bool STAGED, int D>
 struct PageRows {
   const WriteArgs& a;
   const T* stage;  // x's rows, then the residual's
-  int sub, group;
+  int sub, group, d;
   bool in_row;
   // Eight elements of row src (of the page) of x, and of the residual.
   __device__ __forceinline__ void load(const Entry& e, int src, Eight<T>& x, Eight<T>& r) const {
@@ -464,9 +467,9 @@ struct PageRows {
       return;
     }
     if constexpr (STAGED) {
-      const T* const p = stage + src * a.d + sub * 8;
+      const T* const p = stage + src * d + sub * 8;
       x.take(p);
-      if constexpr (SUM) r.take(p + (a.d << a.page_shift));
+      if constexpr (SUM) r.take(p + (d << a.page_shift));
     } else {
       const int64_t at = e.at + src * a.stride_tok + sub * 8;
       x.load(static_cast<const T*>(a.x) + at);
@@ -482,8 +485,8 @@ struct ExactRow {
   double h[8], factor, top;
   bool bad;
 };
-template <typename T, bool SUM, bool WEIGHT, bool STAGED>
-__device__ __forceinline__ void exact_row(const PageRows<T, SUM, WEIGHT, STAGED>& rows, const Entry& e, int src,
+template <typename T, bool SUM, bool WEIGHT, bool STAGED, int D>
+__device__ __forceinline__ void exact_row(const PageRows<T, SUM, WEIGHT, STAGED, D>& rows, const Entry& e, int src,
                                           float near, bool full, ExactRow& o) {
   const WriteArgs& a = rows.a;
   Eight<T> x, r;
@@ -518,7 +521,7 @@ __device__ __forceinline__ void exact_row(const PageRows<T, SUM, WEIGHT, STAGED>
   o.factor = 1.0;
   o.bad = false;
   if (!full) {
-    const double f = near, v = a.norm == TMS_NORM_RMS ? s * (1.0 / a.d) + a.eps : s;
+    const double f = near, v = a.norm == TMS_NORM_RMS ? s * (1.0 / rows.d) + a.eps : s;
     if (a.norm != TMS_NORM_NONE) o.factor = f + 0.5 * f * (1.0 - v * f * f);
     return;
   }
@@ -526,14 +529,15 @@ __device__ __forceinline__ void exact_row(const PageRows<T, SUM, WEIGHT, STAGED>
     const double n = sqrt(s);
     o.factor = 1.0 / (n > a.eps ? n : static_cast<double>(a.eps));
   } else if (a.norm == TMS_NORM_RMS) {
-    o.factor = 1.0 / sqrt(s / a.d + a.eps);
+    o.factor = 1.0 / sqrt(s / rows.d + a.eps);
   }
   o.bad = !(finite(s) && finite(o.top * o.factor));
 }
 
-template <typename T, bool SUM, bool WEIGHT, bool STAGED>
+template <typename T, bool SUM, bool WEIGHT, bool STAGED, int D>
 __global__ void __launch_bounds__(write_threads<T, SUM, STAGED>(), 768 / write_threads<T, SUM, STAGED>())
-page_write_kernel(const WriteArgs a, int group) {
+page_write_kernel(const WriteArgs a, int lanes) {
+  const int d = D > 0 ? D : a.d, group = D > 0 ? D / 8 : lanes;
   constexpr int kWriteThreads = write_threads<T, SUM, STAGED>();
   constexpr uint32_t kAllWarp = 0xffffffffu;
   constexpr int kWarps = kWriteThreads / 32;
@@ -546,9 +550,9 @@ page_write_kernel(const WriteArgs a, int group) {
   const int page = 1 << a.page_shift;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = threadIdx.x & (group - 1), step = kWriteThreads / group, row0 = threadIdx.x / group;
-  const bool in_row = sub < (a.d >> 3);
+  const bool in_row = sub < (d >> 3);
   T* const stages = reinterpret_cast<T*>(stage_bytes);
-  const int stage_elems = (a.d << a.page_shift) * (SUM ? 2 : 1);
+  const int stage_elems = (d << a.page_shift) * (SUM ? 2 : 1);
   Eight<T> wt;
   wt.zero();
   bool odd_weight = false;
@@ -557,7 +561,7 @@ page_write_kernel(const WriteArgs a, int group) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) odd_weight |= !(fabsf(wt.at(j)) <= 1e30f);
   }
-  const float per_d = 1.f / a.d;
+  const float per_d = 1.f / d;
   // After the sums below a lane has those of `held` of its four rows, from row number `mine` on.
   const int held = group == 2 ? 2 : 1;
   const int mine = group == 2 ? (sub & 1) * 2 : (sub & 1) * 2 + (sub >> 1 & 1);
@@ -583,22 +587,22 @@ page_write_kernel(const WriteArgs a, int group) {
   };
   // This thread's part of every row it takes: the same lanes copy a row that read it.
   const int64_t row_jump = step * a.stride_tok, my_from = row0 * a.stride_tok + sub * 8;
-  const uint32_t my_to = smem_u32(stage_bytes) + (row0 * a.d + sub * 8) * static_cast<uint32_t>(sizeof(T));
-  const uint32_t to_jump = step * a.d * static_cast<uint32_t>(sizeof(T));
+  const uint32_t my_to = smem_u32(stage_bytes) + (row0 * d + sub * 8) * static_cast<uint32_t>(sizeof(T));
+  const uint32_t to_jump = step * d * static_cast<uint32_t>(sizeof(T));
   auto fetch = [&](const Entry& e, int which) {  // the entry's rows into a stage
     const int count = e.count < e.limit ? e.count : e.limit;
     uint32_t to = my_to + which * stage_elems * static_cast<uint32_t>(sizeof(T));
     const T* from = static_cast<const T*>(a.x) + e.at + my_from;
     const T* from_res = static_cast<const T*>(a.residual) + e.at + my_from;
-    const uint32_t res = (a.d << a.page_shift) * static_cast<uint32_t>(sizeof(T));
+    const uint32_t res = (d << a.page_shift) * static_cast<uint32_t>(sizeof(T));
     if (!in_row) return;
     for (int row = row0 + (count - row0 + step - 1) / step * step; row < e.count; row += step) {  // rows x does not have
       if (row < count) continue;
-      T* const p = stages + which * stage_elems + row * a.d + sub * 8;
+      T* const p = stages + which * stage_elems + row * d + sub * 8;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         p[i] = T(0.f);
-        if constexpr (SUM) p[(a.d << a.page_shift) + i] = T(0.f);
+        if constexpr (SUM) p[(d << a.page_shift) + i] = T(0.f);
       }
     }
     for (int row = row0; row < count; row += step, to += to_jump, from += row_jump) {
@@ -625,7 +629,7 @@ page_write_kernel(const WriteArgs a, int group) {
     if constexpr (STAGED) fetch(entries[after], now ^ 1);
     const Entry e = entries[at];
     if (e.count == 0) continue;  // the same for the whole CTA
-    const PageRows<T, SUM, WEIGHT, STAGED> rows{a, stages + now * stage_elems, sub, group, in_row};
+    const PageRows<T, SUM, WEIGHT, STAGED, D> rows{a, stages + now * stage_elems, sub, group, d, in_row};
 
     float top = 0.f;
     bool odd = odd_weight;
@@ -741,7 +745,7 @@ page_write_kernel(const WriteArgs a, int group) {
     const bool plain = !odd && usual(scale);
     const float inverse = __frcp_rn(scale);
     if (threadIdx.x == 0) a.scales[e.id] = scale;
-    uint8_t* const out = a.codes + (e.id << a.page_shift) * a.d + sub * 8;
+    uint8_t* const out = a.codes + (e.id << a.page_shift) * d + sub * 8;
     for (int r0 = row0, b = 0; b < page; r0 += 4 * step, b += 4 * step) {  // the same turns for all lanes
       uint32_t unsure = 0;
 #pragma unroll
@@ -780,7 +784,7 @@ page_write_kernel(const WriteArgs a, int group) {
             unsure |= 1u << i;
           }
         }
-        if (in_row) *reinterpret_cast<uint2*>(out + row * a.d) = make_uint2(word[0], word[1]);
+        if (in_row) *reinterpret_cast<uint2*>(out + row * d) = make_uint2(word[0], word[1]);
       }
       // Rows that fp32 is not sure of, again.
       uint32_t again = __reduce_or_sync(kAllWarp, unsure);
@@ -798,7 +802,7 @@ page_write_kernel(const WriteArgs a, int group) {
           const uint32_t code = bad ? 0x7fu : scale > 0.f ? e4m3_of_double(exact.h[j] * exact.factor / scale) : 0u;
           word[j >> 2] |= code << (8 * (j & 3));
         }
-        *reinterpret_cast<uint2*>(out + row * a.d) = make_uint2(word[0], word[1]);
+        *reinterpret_cast<uint2*>(out + row * d) = make_uint2(word[0], word[1]);
       }
     }
   }
@@ -812,16 +816,19 @@ cudaError_t launch_write_as(const WriteArgs& a, const DeviceInfo* dev, cudaStrea
   const int input = (a.d << a.page_shift) * static_cast<int>(sizeof(T)) * (SUM ? 2 : 1);
   const bool staged = input <= kStageBytes;
   // As many CTAs as fit at a time: each then has its next page on the way while it works on one.
-  const int fit = staged ? dev->max_smem_optin / (2 * input + 2048) : 16;
+  const int fit = staged ? dev->max_smem_optin / (2 * input + kStaticBytes) : 16;
   const int64_t most = static_cast<int64_t>(dev->num_sms) * (fit < 16 ? fit : 16);
   const unsigned blocks = static_cast<unsigned>(a.page_cap < most ? a.page_cap : most);
   if (staged) {
-    auto kern = page_write_kernel<T, SUM, WEIGHT, true>;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStageBytes);
-    if (e != cudaSuccess) return e;
+    // A constant width where it is the usual one: see the kernel's figures.
+    auto kern = a.d == 128 ? page_write_kernel<T, SUM, WEIGHT, true, 128> : page_write_kernel<T, SUM, WEIGHT, true, 0>;
+    if (2 * input + kStaticBytes > 48 * 1024) {  // more than a launch may have unasked
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStageBytes);
+      if (e != cudaSuccess) return e;
+    }
     kern<<<blocks, write_threads<T, SUM, true>(), 2 * input, st>>>(a, group);
   } else {
-    page_write_kernel<T, SUM, WEIGHT, false><<<blocks, write_threads<T, SUM, false>(), 0, st>>>(a, group);
+    page_write_kernel<T, SUM, WEIGHT, false, 0><<<blocks, write_threads<T, SUM, false>(), 0, st>>>(a, group);
   }
   return cudaGetLastError();
 }
