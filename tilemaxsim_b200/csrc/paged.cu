@@ -402,7 +402,7 @@ struct Eight {
   }
 };
 
-// One page at a time a CTA of two or four warps, the next page on its way into shared memory (cp.async)
+// One page at a time a CTA of one, two or four warps, the next page on its way into shared memory (cp.async)
 // meanwhile; a group of 2 to 32 lanes takes a row, eight elements a lane. The input is read from
 // memory once and the codes are written once, which bounds the kernel. Pages of more than
 // kStageBytes of input are read twice instead, the second time from the caches.
@@ -425,11 +425,12 @@ struct Eight {
 __device__ __forceinline__ double max_keep_nan(double x, double y) { return y <= x || x != x ? x : y; }
 __device__ __forceinline__ bool usual(float v) { return v >= 1e-30f && v <= 1e30f; }
 
-// Threads of a CTA: 64 where a page's input is 16-bit values alone; 128 where twice the input leaves
-// room for half as many CTAs (1,024 documents with a residual: 72 us with 64, 61 with 128), and
-// where pages are not staged.
-template <typename T, bool SUM, bool STAGED>
-constexpr int write_threads() { return sizeof(T) == 2 && !SUM && STAGED ? 64 : 128; }
+// Threads of a CTA: 32 where a page's input is 4 KB at most, 64 up to 8 KB, else 128: as many CTAs as
+// shared memory has stages for then have warps enough, and few warps a page wait for one another
+// little. 3.64M tokens of bf16: d = 64 294 us with 32 threads, 413 with 64; pages of 16 478 and 702;
+// pages of 32 523-610 with 32, 456 with 64, 555 with 128. 1,024 documents with a residual (16 KB a page):
+// 51 us with 64, 43 with 128.
+constexpr int write_threads(int input) { return input <= 4096 ? 32 : input <= 8192 ? 64 : 128; }
 constexpr int kStaticBytes = 2048;       // a CTA's other shared memory, at most
 constexpr int kStageBytes = 24 * 1024;  // most input of a page (x and residual) that is staged
 
@@ -534,11 +535,10 @@ __device__ __forceinline__ void exact_row(const PageRows<T, SUM, WEIGHT, STAGED,
   o.bad = !(finite(s) && finite(o.top * o.factor));
 }
 
-template <typename T, bool SUM, bool WEIGHT, bool STAGED, int D>
-__global__ void __launch_bounds__(write_threads<T, SUM, STAGED>(), 768 / write_threads<T, SUM, STAGED>())
+template <typename T, bool SUM, bool WEIGHT, bool STAGED, int D, int kWriteThreads>
+__global__ void __launch_bounds__(kWriteThreads, 768 / kWriteThreads)
 page_write_kernel(const WriteArgs a, int lanes) {
   const int d = D > 0 ? D : a.d, group = D > 0 ? D / 8 : lanes;
-  constexpr int kWriteThreads = write_threads<T, SUM, STAGED>();
   constexpr uint32_t kAllWarp = 0xffffffffu;
   constexpr int kWarps = kWriteThreads / 32;
   extern __shared__ __align__(16) uint8_t stage_bytes[];
@@ -809,28 +809,45 @@ page_write_kernel(const WriteArgs a, int lanes) {
   if constexpr (STAGED) cp_async_wait_all();
 }
 
+template <typename T, bool SUM, bool WEIGHT, int D, int THREADS>
+cudaError_t launch_staged(const WriteArgs& a, int group, unsigned blocks, int input, cudaStream_t st) {
+  // A constant width has pages of 16 rows at least: fewer threads than those take are not reached.
+  if constexpr (D > 0 && THREADS < write_threads(D * 16 * static_cast<int>(sizeof(T)) * (SUM ? 2 : 1))) {
+    return cudaErrorInvalidValue;
+  } else {
+    auto kern = page_write_kernel<T, SUM, WEIGHT, true, D, THREADS>;
+    if (2 * input + kStaticBytes > 48 * 1024) {  // more than a launch may have unasked
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStageBytes);
+      if (e != cudaSuccess) return e;
+    }
+    kern<<<blocks, THREADS, 2 * input, st>>>(a, group);
+    return cudaGetLastError();
+  }
+}
+
 template <typename T, bool SUM, bool WEIGHT>
 cudaError_t launch_write_as(const WriteArgs& a, const DeviceInfo* dev, cudaStream_t st) {
   int group = 2;  // lanes of a row
   while (group * 8 < a.d) group <<= 1;
   const int input = (a.d << a.page_shift) * static_cast<int>(sizeof(T)) * (SUM ? 2 : 1);
   const bool staged = input <= kStageBytes;
+  const int threads = staged ? write_threads(input) : 128;
   // As many CTAs as fit at a time: each then has its next page on the way while it works on one.
-  const int fit = staged ? dev->max_smem_optin / (2 * input + kStaticBytes) : 16;
-  const int64_t most = static_cast<int64_t>(dev->num_sms) * (fit < 16 ? fit : 16);
+  const int fit = staged ? dev->max_smem_optin / (2 * input + kStaticBytes) : 16, room = staged ? 768 / threads : 16;
+  const int64_t most = static_cast<int64_t>(dev->num_sms) * (fit < room ? fit : room);
   const unsigned blocks = static_cast<unsigned>(a.page_cap < most ? a.page_cap : most);
-  if (staged) {
-    // A constant width where it is the usual one: see the kernel's figures.
-    auto kern = a.d == 128 ? page_write_kernel<T, SUM, WEIGHT, true, 128> : page_write_kernel<T, SUM, WEIGHT, true, 0>;
-    if (2 * input + kStaticBytes > 48 * 1024) {  // more than a launch may have unasked
-      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStageBytes);
-      if (e != cudaSuccess) return e;
-    }
-    kern<<<blocks, write_threads<T, SUM, true>(), 2 * input, st>>>(a, group);
-  } else {
-    page_write_kernel<T, SUM, WEIGHT, false, 0><<<blocks, write_threads<T, SUM, false>(), 0, st>>>(a, group);
+  if (!staged) {
+    page_write_kernel<T, SUM, WEIGHT, false, 0, 128><<<blocks, 128, 0, st>>>(a, group);
+    return cudaGetLastError();
   }
-  return cudaGetLastError();
+  if (a.d == 128) {  // a constant width where it is the usual one: see the kernel's figures
+    return threads == 32   ? launch_staged<T, SUM, WEIGHT, 128, 32>(a, group, blocks, input, st)
+           : threads == 64 ? launch_staged<T, SUM, WEIGHT, 128, 64>(a, group, blocks, input, st)
+                           : launch_staged<T, SUM, WEIGHT, 128, 128>(a, group, blocks, input, st);
+  }
+  return threads == 32   ? launch_staged<T, SUM, WEIGHT, 0, 32>(a, group, blocks, input, st)
+         : threads == 64 ? launch_staged<T, SUM, WEIGHT, 0, 64>(a, group, blocks, input, st)
+                         : launch_staged<T, SUM, WEIGHT, 0, 128>(a, group, blocks, input, st);
 }
 
 template <typename T>
