@@ -156,6 +156,15 @@ def test_write(page, d, lengths, norm, residual, weight, dtype, cuda_device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("norm,residual,weight", [("l2", False, False), ("rms", True, True), ("rms", False, True), ("none", False, False)])
+@pytest.mark.parametrize("page,d", [(16, 128), (64, 128), (128, 128), (16, 64), (128, 16), (16, 256), (32, 256)])
+def test_write_by_the_bytes_of_a_page(page, d, norm, residual, weight, dtype, cuda_device):
+    """A page's input decides how many warps take it, and whether it is staged: 512 bytes to 128 KB."""
+    lengths = [page * 3 + 1, 0, 1, page, page - 1] + torch.randint(0, 3 * page, (40,), generator=_rng(d)).tolist()
+    test_write(page, d, lengths, norm, residual, weight, dtype, cuda_device)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_write_padded_batch_and_strides(dtype, cuda_device):
     """A padded batch with garbage (NaN) behind each document, and views with other strides, write the
     same pages as the ragged tokens."""
@@ -456,6 +465,40 @@ def test_scores_token_widths(bq, page, dtype, d, cuda_device):
     _check_scores(got[:, pick], Q, [docs[i] for i in pick])
     for i in range(0, bq, 7):  # alone or in a batch: within the bound of the kernel's own arithmetic
         _check_scores(paged_maxsim(Q[i:i + 1], codes, scales, t)[:, pick], Q[i:i + 1], [docs[j] for j in pick])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bq,nq", [(1, 32), (1, 5), (2, 32), (1, 64), (3, 32)])
+@pytest.mark.parametrize("page,n,hi", [(16, 700, 90), (32, 700, 90), (64, 300, 400), (128, 300, 400), (16, 5, 3000), (32, 5, 3000)])
+def test_scores_two_tokens_a_row(page, n, hi, bq, nq, dtype, cuda_device):
+    """d = 64: two tokens share 128 bytes. Streams of many tiles, documents cut by streams and ranges."""
+    from tilemaxsim_b200 import paged_maxsim
+    lengths = torch.randint(0, hi, (n,), generator=_rng(page + n)).tolist()
+    t, codes, scales, docs = _corpus(lengths, page, 64, bq + nq)
+    Q = _queries(bq, nq, 64, 7, dtype)
+    got = paged_maxsim(Q, codes, scales, t)
+    _check_scores(got, Q, docs)
+    assert torch.equal(got, paged_maxsim(Q, codes, scales, t))
+
+
+@pytest.mark.parametrize("bq", [1, 2])
+def test_scores_two_tokens_a_row_which_is_which(bq, cuda_device):
+    """Every token of a document in its turn the only one that a query finds, a NaN page beside it."""
+    from tilemaxsim_b200 import page_write, paged_maxsim
+    page, n = 16, 64
+    t, n_pages = _layout([n, 16, n], page, 3)
+    x = torch.zeros(n + 16 + n, 64)
+    x[:n] = torch.eye(64)
+    x[n:n + 16] = float("nan")
+    x[n + 16:] = torch.eye(64).flip(0) * 0.5
+    codes = torch.zeros(n_pages, page, 64, device=cuda_device).to(torch.float8_e4m3fn)
+    scales = torch.zeros(n_pages, device=cuda_device)
+    page_write(x.half().cuda(), t, codes, scales, norm="none")
+    Q = torch.eye(64).view(64 // (32 * bq), bq, 32, 64).half().cuda()
+    for q in Q:
+        got = paged_maxsim(q, codes, scales, t).cpu()
+        assert torch.equal(got[:, 0], torch.full((bq,), 32.0)) and got[:, 1].isnan().all()
+        assert torch.equal(got[:, 2], torch.full((bq,), 16.0))
 
 
 @pytest.mark.parametrize("bq,page", [(1, 32), (2, 16), (4, 64), (20, 32)])
