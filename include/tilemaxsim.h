@@ -68,6 +68,8 @@ extern "C" {
 
 #define TMS_PAGED_MAX_D 256 /* widest token of a paged corpus */
 
+#define TMS_TOPK_MAX_IDS 16384 /* longest row of tms_topk with explicit ids */
+
 /* dense output modes */
 #define TMS_OUT_SCORE 0     /* out[q * n_docs + doc] = sum_i max_j <Q_qi, D_j>                 */
 #define TMS_OUT_TOKEN_MAX 1 /* out[(q * n_docs + doc) * nq + i] = max_j <Q_qi, D_j> (V1 output) */
@@ -203,7 +205,8 @@ TMS_API size_t tms_topk_workspace_size(int64_t rows, int64_t n, int64_t k);
 
 /* Per row r of scores (rows, n) fp32 with row stride ld: the k best (score descending, then id
  * ascending; NaN ranks last) -> out_vals (rows, k), out_ids (rows, k) int64. The id of column c is
- * ids_in[r*ld_ids + c] when ids_in != NULL, else c + id_base. k <= 2048 and k <= n. */
+ * ids_in[r*ld_ids + c] when ids_in != NULL, else c + id_base. k <= 2048 and k <= n; with ids_in,
+ * n <= TMS_TOPK_MAX_IDS. */
 TMS_API int tms_topk(const float* scores, int64_t rows, int64_t n, int64_t ld, int64_t k,
              const int64_t* ids_in, int64_t ld_ids, int64_t id_base, float* out_vals,
              int64_t* out_ids, void* workspace, size_t workspace_bytes, void* stream);

@@ -28,6 +28,7 @@ TMS_F16, TMS_BF16, TMS_F32 = 0, 1, 2
 TMS_OUT_SCORE, TMS_OUT_TOKEN_MAX = 0, 1
 TMS_NORM_NONE, TMS_NORM_L2, TMS_NORM_RMS = 0, 1, 2
 TMS_PAGED_MAX_D = 256
+TMS_TOPK_MAX_IDS = 16384
 TMS_PQ_FAST, TMS_PQ_EXACT, TMS_PQ_PRECISE = 0, 1, 2
 
 DTYPE_CODE = {torch.float16: TMS_F16, torch.bfloat16: TMS_BF16, torch.float32: TMS_F32}

@@ -16,7 +16,7 @@ namespace tms {
 namespace {
 
 constexpr int kTopkThreads = 1024;
-constexpr int kSortMax = 16384;  // elements sorted whole in shared memory (12 B each)
+constexpr int kSortMax = TMS_TOPK_MAX_IDS;  // elements sorted whole in shared memory (12 B each)
 constexpr int kMaxK = 2048;
 
 // Order-preserving key: larger float -> larger key; every NaN -> 0 (ranks last).

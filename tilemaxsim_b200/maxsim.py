@@ -117,7 +117,7 @@ def maxsim_batched(Qb: torch.Tensor, D_tokens: torch.Tensor, doc_offsets: torch.
 def topk(scores: torch.Tensor, k: int, ids: torch.Tensor | None = None, id_base: int = 0
          ) -> tuple[torch.Tensor, torch.Tensor]:
     """Per-row top-k of (rows, n) fp32 scores, ordered by score descending then id ascending (NaN
-    last). Ids are column + id_base, or ids[r, c] when given. Returns (values (rows, k) fp32,
+    last). Ids are column + id_base, or ids[r, c] when given (rows of at most 16,384 then). Returns (values (rows, k) fp32,
     ids (rows, k) int64)."""
     lib = _lib.load()
     single = scores.dim() == 1

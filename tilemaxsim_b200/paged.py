@@ -418,11 +418,17 @@ class PagedCorpus:
 
     def search(self, Qb: torch.Tensor, k: int, doc_ids: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The k best documents of each query, of all or of the candidates doc_ids (n,): scores
-        (B_q, k) fp32 and ids (B_q, k) int64, by score descending and id ascending."""
-        scores = self.score_queries(Qb, doc_ids)
+        (B_q, k) fp32 and ids (B_q, k) int64, by score descending and id ascending. An id that comes
+        twice among the candidates is ranked twice."""
         if doc_ids is None:
-            return topk(scores, k)
-        return topk(scores, k, ids=doc_ids.to(torch.int64).expand(scores.shape).contiguous())
+            return topk(self.score_queries(Qb), k)
+        ids = _ints(doc_ids, torch.int64, "doc_ids")
+        if ids.numel() <= _lib.TMS_TOPK_MAX_IDS:
+            scores = self.score_queries(Qb, ids)
+            return topk(scores, k, ids=ids.expand(scores.shape).contiguous())
+        ids = ids.sort().values  # columns ascend with the id: the tie rule carries over
+        vals, col = topk(self.score_queries(Qb, ids), k)
+        return vals, ids[col]
 
     def tokens(self, doc_ids: torch.Tensor | list[int], dtype: torch.dtype = torch.float16
                ) -> tuple[torch.Tensor, torch.Tensor]:
