@@ -211,6 +211,18 @@ TMS_API int tms_topk(const float* scores, int64_t rows, int64_t n, int64_t ld, i
              const int64_t* ids_in, int64_t ld_ids, int64_t id_base, float* out_vals,
              int64_t* out_ids, void* workspace, size_t workspace_bytes, void* stream);
 
+TMS_API size_t tms_topk_docs_workspace_size(int64_t rows, int64_t n, int64_t k);
+
+/* tms_topk over the documents of a store with the given lengths (n_docs). Column c is document
+ * doc_ids[c], or c when doc_ids == NULL. Columns of documents without tokens rank after all others, a
+ * NaN's included, by id, and those of ids outside [0, n_docs) after them. Both come back with -inf, and
+ * with id -1 but for documents of doc_ids without tokens, which keep their ids. With doc_ids,
+ * rows of more than TMS_TOPK_MAX_IDS break ties by column: give such ids in ascending order, those
+ * outside last. The workspace is 16-byte aligned. */
+TMS_API int tms_topk_docs(const float* scores, int64_t rows, int64_t n, int64_t ld, int64_t k,
+                          const int64_t* doc_ids, const int64_t* lengths, int64_t n_docs, float* out_vals,
+                          int64_t* out_ids, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- candidate generation (IVF probe) */
 /* No reference function: the reference reaches a candidate stage only through external searchers
  * (PLAID's dense_search, src/plaid_integration_benchmark.py:186-211; WARP, baselines/bench_warp.py).

@@ -74,6 +74,8 @@ SIGNATURES = {
     "tms_paged_maxsim": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp,
                                 _vp, _sz, _vp]),
     "tms_topk_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "tms_topk_docs_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "tms_topk_docs": (_i32, [_vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _sz, _vp]),
     "tms_topk": (_i32, [_vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
 }
 

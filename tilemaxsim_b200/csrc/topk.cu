@@ -9,6 +9,9 @@
 //    and how many of its ties are needed; one more pass gathers every key > K* and, through an
 //    ordered block scan, the lowest-index ties; the k candidates are then bitonic-sorted.
 // Each pass reads the row once (the rows of a score matrix stay L2-resident between passes).
+//
+// The documents of a store (tms_topk_docs, DOCS below) carry a mark in their id: columns without
+// tokens rank after all others, a NaN's included, in either kernel.
 #include "tms_device.cuh"
 #include "tms_internal.h"
 
@@ -28,6 +31,26 @@ __device__ __forceinline__ uint32_t f2key(float f) {
 __device__ __forceinline__ float key2f(uint32_t k) {
   const uint32_t b = (k & 0x80000000u) ? (k & 0x7fffffffu) : ~k;
   return __uint_as_float(b);  // key 0 decodes to 0xffffffff, a NaN
+}
+
+// What tms_topk_docs ranks a column by: its document's id; that plus kGone where the document has no
+// tokens; kOutside where there is no such document. As ids these rank last among the keys of a NaN.
+constexpr int64_t kGone = int64_t(1) << 62, kOutside = INT64_MAX;
+
+__global__ void __launch_bounds__(256) mark_docs_kernel(const int64_t* __restrict__ doc_ids, int64_t n,
+                                                        const int64_t* __restrict__ lengths, int64_t n_docs,
+                                                        int64_t* __restrict__ marked) {
+  for (int64_t c = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; c < n;
+       c += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t id = doc_ids ? doc_ids[c] : c;
+    marked[c] = id < 0 || id >= n_docs ? kOutside : lengths[id] > 0 ? id : id + kGone;
+  }
+}
+
+// A ranked column as tms_topk_docs returns it.
+__device__ __forceinline__ void put_doc(float v, int64_t marked, bool name_gone, float* val, int64_t* id) {
+  *val = marked >= kGone ? -__builtin_huge_valf() : v;
+  *id = marked < kGone ? marked : name_gone && marked != kOutside ? marked - kGone : -1;
 }
 
 // true if (ka, ia) ranks before (kb, ib)
@@ -64,10 +87,12 @@ __device__ __forceinline__ int next_pow2(int x) {
   return p;
 }
 
+// DOCS: ids_in are marked ids, and name_gone says whether those of documents without tokens come back.
+template <bool DOCS>
 __global__ void __launch_bounds__(kTopkThreads)
     topk_sort_kernel(const float* __restrict__ scores, int64_t n, int64_t ld, int k,
                      const int64_t* __restrict__ ids_in, int64_t ld_ids, int64_t id_base,
-                     float* __restrict__ out_vals, int64_t* __restrict__ out_ids) {
+                     float* __restrict__ out_vals, int64_t* __restrict__ out_ids, bool name_gone) {
   extern __shared__ __align__(16) uint8_t sm[];
   const int P = next_pow2(static_cast<int>(n));
   int64_t* ids = reinterpret_cast<int64_t*>(sm);
@@ -78,6 +103,7 @@ __global__ void __launch_bounds__(kTopkThreads)
     if (i < n) {
       keys[i] = f2key(s[i]);
       ids[i] = ids_in ? ids_in[row * ld_ids + i] : id_base + i;
+      if (DOCS && ids[i] >= kGone) keys[i] = 0u;
     } else {
       keys[i] = 0u;
       ids[i] = INT64_MAX;
@@ -86,8 +112,12 @@ __global__ void __launch_bounds__(kTopkThreads)
   __syncthreads();
   bitonic_sort(keys, ids, P);
   for (int i = threadIdx.x; i < k; i += blockDim.x) {
-    out_vals[row * k + i] = key2f(keys[i]);
-    out_ids[row * k + i] = ids[i];
+    if constexpr (DOCS) {
+      put_doc(key2f(keys[i]), ids[i], name_gone, out_vals + row * k + i, out_ids + row * k + i);
+    } else {
+      out_vals[row * k + i] = key2f(keys[i]);
+      out_ids[row * k + i] = ids[i];
+    }
   }
 }
 
@@ -133,10 +163,14 @@ __global__ void __launch_bounds__(kTopkThreads)
   }
 }
 
+// DOCS: `marked` holds every column's marked id. With several slices these come out as they are, for the
+// merge.
+template <bool DOCS>
 __global__ void __launch_bounds__(kTopkThreads)
     topk_select_kernel(const float* __restrict__ scores, int64_t n, int64_t ld, int k,
                        int64_t id_base, float* __restrict__ out_vals,
-                       int64_t* __restrict__ out_ids, int64_t chunk, int n_chunks) {
+                       int64_t* __restrict__ out_ids, int64_t chunk, int n_chunks,
+                       const int64_t* __restrict__ marked, bool name_gone) {
   __shared__ uint32_t hist[256];
   __shared__ uint32_t s_prefix, s_mask, s_remaining;
   __shared__ uint32_t s_gt_pos, s_taken;
@@ -149,6 +183,12 @@ __global__ void __launch_bounds__(kTopkThreads)
   const int64_t row = blockIdx.x;
   const int64_t r = row / n_chunks, c = row - r * n_chunks;
   const float* s = scores + r * ld + c * chunk;
+  const int64_t* const marks = DOCS ? marked + c * chunk : nullptr;
+  auto key_at = [&](int64_t i) {  // documents without tokens below a NaN, which key 1 stands for too
+    const uint32_t key = f2key(__ldg(s + i));
+    if constexpr (DOCS) return __ldg(marks + i) >= kGone ? 0u : key == 0u ? 1u : key;
+    else return key;
+  };
   const int64_t n_all = n;
   n = (n_all - c * chunk < chunk) ? n_all - c * chunk : chunk;
   id_base += c * chunk;
@@ -174,7 +214,7 @@ __global__ void __launch_bounds__(kTopkThreads)
     __syncthreads();
     const uint32_t prefix = s_prefix, mask = s_mask;
     for (int64_t i = tid; i < n; i += blockDim.x) {
-      const uint32_t key = f2key(__ldg(s + i));
+      const uint32_t key = key_at(i);
       if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
     }
     __syncthreads();
@@ -204,7 +244,7 @@ __global__ void __launch_bounds__(kTopkThreads)
     uint32_t key = 0;
     bool gt = false, eq = false;
     if (i < n) {
-      key = f2key(__ldg(s + i));
+      key = key_at(i);
       gt = key > kth;
       eq = key == kth;
     }
@@ -249,6 +289,17 @@ __global__ void __launch_bounds__(kTopkThreads)
   __syncthreads();
   bitonic_sort(cand_keys, cand_ids, P);
   for (int i = tid; i < k_out; i += blockDim.x) {
+    if constexpr (DOCS) {
+      const int64_t id = i < k ? marks[cand_ids[i]] : kOutside;
+      const float v = key2f(i < k ? cand_keys[i] : 0u);
+      if (n_chunks == 1) {
+        put_doc(v, id, name_gone, out_vals + row * k_out + i, out_ids + row * k_out + i);
+      } else {
+        out_vals[row * k_out + i] = v;
+        out_ids[row * k_out + i] = id;
+      }
+      continue;
+    }
     out_vals[row * k_out + i] = i < k ? key2f(cand_keys[i]) : key2f(0u);
     out_ids[row * k_out + i] = i < k ? cand_ids[i] + id_base : INT64_MAX;
   }
@@ -278,6 +329,52 @@ extern "C" size_t tms_topk_workspace_size(int64_t rows, int64_t n, int64_t k) {
   return c > 1 ? static_cast<size_t>(rows * c * k) * 12 + 256 : 0;
 }
 
+namespace {
+// ids_in: explicit ids of the columns, ld_ids from one row to the next, for rows of at most kSortMax.
+// DOCS: marked ids (n), the same for every row, whatever n is.
+template <bool DOCS>
+int launch_topk(const float* scores, int64_t rows, int64_t n, int64_t ld, int64_t k, const int64_t* ids_in,
+                int64_t ld_ids, int64_t id_base, bool name_gone, float* out_vals, int64_t* out_ids, void* workspace,
+                size_t workspace_bytes, cudaStream_t st) {
+  if (n <= kSortMax) {
+    int P = 1;
+    while (P < n) P <<= 1;
+    const size_t smem = static_cast<size_t>(P) * 12;
+    if (cudaFuncSetAttribute(topk_sort_kernel<DOCS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem)) != cudaSuccess)
+      return TMS_ERR_CUDA;
+    topk_sort_kernel<DOCS><<<static_cast<unsigned>(rows), kTopkThreads, smem, st>>>(
+        scores, n, ld, static_cast<int>(k), ids_in, ld_ids, id_base, out_vals, out_ids, name_gone);
+    return cuda_status(cudaGetLastError());
+  }
+  const int c = topk_chunks(rows, n, k);
+  if (c > 1 && workspace && workspace_bytes >= tms_topk_workspace_size(rows, n, k) &&
+      rows * c <= 0x7fffffffLL) {
+    // slice top-k into the workspace, then one sort-merge per row (ids carried explicitly)
+    int64_t* cand_ids = reinterpret_cast<int64_t*>(
+        (reinterpret_cast<uintptr_t>(workspace) + 15) & ~static_cast<uintptr_t>(15));
+    float* cand_vals = reinterpret_cast<float*>(cand_ids + rows * c * k);
+    const int64_t chunk = (n + c - 1) / c;
+    topk_select_kernel<DOCS><<<static_cast<unsigned>(rows * c), kTopkThreads, 0, st>>>(
+        scores, n, ld, static_cast<int>(k), id_base, cand_vals, cand_ids, chunk, c, ids_in, name_gone);
+    if (cudaGetLastError() != cudaSuccess) return TMS_ERR_CUDA;
+    const int64_t m = static_cast<int64_t>(c) * k;
+    int P = 1;
+    while (P < m) P <<= 1;
+    const size_t smem = static_cast<size_t>(P) * 12;
+    if (cudaFuncSetAttribute(topk_sort_kernel<DOCS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem)) != cudaSuccess)
+      return TMS_ERR_CUDA;
+    topk_sort_kernel<DOCS><<<static_cast<unsigned>(rows), kTopkThreads, smem, st>>>(
+        cand_vals, m, m, static_cast<int>(k), cand_ids, m, 0, out_vals, out_ids, name_gone);
+    return cuda_status(cudaGetLastError());
+  }
+  topk_select_kernel<DOCS><<<static_cast<unsigned>(rows), kTopkThreads, 0, st>>>(
+      scores, n, ld, static_cast<int>(k), id_base, out_vals, out_ids, n, 1, ids_in, name_gone);
+  return cuda_status(cudaGetLastError());
+}
+}  // namespace
+
 extern "C" int tms_topk(const float* scores, int64_t rows, int64_t n, int64_t ld, int64_t k,
                         const int64_t* ids_in, int64_t ld_ids, int64_t id_base, float* out_vals,
                         int64_t* out_ids, void* workspace, size_t workspace_bytes, void* stream) {
@@ -290,44 +387,37 @@ extern "C" int tms_topk(const float* scores, int64_t rows, int64_t n, int64_t ld
   int status = TMS_OK;
   const DeviceInfo* dev = current_device_info(&status);
   if (!dev) return status;
+  if (ids_in && n > kSortMax) return TMS_ERR_UNSUPPORTED;  // explicit ids are for shard merges (short rows)
+  return launch_topk<false>(scores, rows, n, ld, k, ids_in, ld_ids, id_base, false, out_vals, out_ids, workspace,
+                            workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t tms_topk_docs_workspace_size(int64_t rows, int64_t n, int64_t k) {
+  return n > 0 ? align_up(static_cast<size_t>(n) * sizeof(int64_t), 16) + tms_topk_workspace_size(rows, n, k) : 0;
+}
+
+extern "C" int tms_topk_docs(const float* scores, int64_t rows, int64_t n, int64_t ld, int64_t k,
+                             const int64_t* doc_ids, const int64_t* lengths, int64_t n_docs, float* out_vals,
+                             int64_t* out_ids, void* workspace, size_t workspace_bytes, void* stream) {
+  NvtxRange nvtx_range("tms_topk_docs");
+  if (rows < 0 || n < 0 || k < 0 || ld < n || n_docs < 0) return TMS_ERR_INVALID;
+  if (rows == 0 || k == 0) return TMS_OK;
+  if (k > n || !scores || !out_vals || !out_ids || (n_docs > 0 && !lengths)) return TMS_ERR_INVALID;
+  if (k > kMaxK || rows > 0x7fffffffLL || n_docs > kGone) return TMS_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < tms_topk_docs_workspace_size(rows, n, k)) return TMS_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return TMS_ERR_INVALID;
+  int status = TMS_OK;
+  const DeviceInfo* dev = current_device_info(&status);
+  if (!dev) return status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (n <= kSortMax) {
-    int P = 1;
-    while (P < n) P <<= 1;
-    const size_t smem = static_cast<size_t>(P) * 12;
-    if (cudaFuncSetAttribute(topk_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem)) != cudaSuccess)
-      return TMS_ERR_CUDA;
-    topk_sort_kernel<<<static_cast<unsigned>(rows), kTopkThreads, smem, st>>>(
-        scores, n, ld, static_cast<int>(k), ids_in, ld_ids, id_base, out_vals, out_ids);
-    return cuda_status(cudaGetLastError());
-  }
-  if (ids_in) return TMS_ERR_UNSUPPORTED;  // explicit ids are for shard merges (short rows)
-  const int c = topk_chunks(rows, n, k);
-  if (c > 1 && workspace && workspace_bytes >= tms_topk_workspace_size(rows, n, k) &&
-      rows * c <= 0x7fffffffLL) {
-    // slice top-k into the workspace, then one sort-merge per row (ids carried explicitly)
-    int64_t* cand_ids = reinterpret_cast<int64_t*>(
-        (reinterpret_cast<uintptr_t>(workspace) + 15) & ~static_cast<uintptr_t>(15));
-    float* cand_vals = reinterpret_cast<float*>(cand_ids + rows * c * k);
-    const int64_t chunk = (n + c - 1) / c;
-    topk_select_kernel<<<static_cast<unsigned>(rows * c), kTopkThreads, 0, st>>>(
-        scores, n, ld, static_cast<int>(k), id_base, cand_vals, cand_ids, chunk, c);
-    if (cudaGetLastError() != cudaSuccess) return TMS_ERR_CUDA;
-    const int64_t m = static_cast<int64_t>(c) * k;
-    int P = 1;
-    while (P < m) P <<= 1;
-    const size_t smem = static_cast<size_t>(P) * 12;
-    if (cudaFuncSetAttribute(topk_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem)) != cudaSuccess)
-      return TMS_ERR_CUDA;
-    topk_sort_kernel<<<static_cast<unsigned>(rows), kTopkThreads, smem, st>>>(
-        cand_vals, m, m, static_cast<int>(k), cand_ids, m, 0, out_vals, out_ids);
-    return cuda_status(cudaGetLastError());
-  }
-  topk_select_kernel<<<static_cast<unsigned>(rows), kTopkThreads, 0, st>>>(
-      scores, n, ld, static_cast<int>(k), id_base, out_vals, out_ids, n, 1);
-  return cuda_status(cudaGetLastError());
+  int64_t* const marked = static_cast<int64_t*>(workspace);
+  const size_t held = align_up(static_cast<size_t>(n) * sizeof(int64_t), 16);
+  const int64_t blocks = (n + 255) / 256, most = static_cast<int64_t>(dev->num_sms) * 8;
+  mark_docs_kernel<<<static_cast<unsigned>(blocks < most ? blocks : most), 256, 0, st>>>(doc_ids, n, lengths, n_docs,
+                                                                                        marked);
+  if (cudaGetLastError() != cudaSuccess) return TMS_ERR_CUDA;
+  return launch_topk<true>(scores, rows, n, ld, k, marked, 0, 0, doc_ids != nullptr, out_vals, out_ids,
+                           static_cast<uint8_t*>(workspace) + held, workspace_bytes - held, st);
 }
 
 extern "C" int tms_topk_pack(const float* vals, const int64_t* ids, int64_t rows, int64_t k,

@@ -21,7 +21,6 @@ import numpy as np
 import torch
 
 from . import _lib
-from .maxsim import topk
 
 PAGE_SIZES = (16, 32, 64, 128)
 _NORMS = {"none": _lib.TMS_NORM_NONE, "l2": _lib.TMS_NORM_L2, "rms": _lib.TMS_NORM_RMS}
@@ -418,17 +417,33 @@ class PagedCorpus:
 
     def search(self, Qb: torch.Tensor, k: int, doc_ids: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The k best documents of each query, of all or of the candidates doc_ids (n,): scores
-        (B_q, k) fp32 and ids (B_q, k) int64, by score descending and id ascending. An id that comes
-        twice among the candidates is ranked twice."""
-        if doc_ids is None:
-            return topk(self.score_queries(Qb), k)
-        ids = _ints(doc_ids, torch.int64, "doc_ids")
-        if ids.numel() <= _lib.TMS_TOPK_MAX_IDS:
-            scores = self.score_queries(Qb, ids)
-            return topk(scores, k, ids=ids.expand(scores.shape).contiguous())
-        ids = ids.sort().values  # columns ascend with the id: the tie rule carries over
-        vals, col = topk(self.score_queries(Qb, ids), k)
-        return vals, ids[col]
+        (B_q, k) fp32 and ids (B_q, k) int64, by score descending (NaN last) and id ascending. An id
+        that comes twice among the candidates is ranked twice. Documents without tokens (removed, or
+        added empty) come after all others with -inf: as id -1 in a search of all documents, by their
+        own ids among candidates, where ids outside the corpus end the list as -1."""
+        if doc_ids is not None:
+            doc_ids = _ints(doc_ids, torch.int64, "doc_ids")
+            if doc_ids.numel() > _lib.TMS_TOPK_MAX_IDS:  # ties go by column there
+                outside = (doc_ids < 0) | (doc_ids >= self.n_docs)
+                doc_ids = doc_ids.masked_fill(outside, torch.iinfo(torch.int64).max).sort().values
+        return self._topk(self.score_queries(Qb, doc_ids), k, doc_ids)
+
+    def _topk(self, scores: torch.Tensor, k: int, doc_ids: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+        lib = _lib.load()
+        single = scores.dim() == 1
+        rows, n = scores.shape if not single else (1, scores.numel())
+        if not 0 < k <= n:
+            raise ValueError(f"k={k} must be in [1, n={n}]")
+        with _lib.on_device(self.device):
+            vals = torch.empty((rows, k), dtype=torch.float32, device=self.device)
+            ids = torch.empty((rows, k), dtype=torch.int64, device=self.device)
+            ws_bytes = lib.tms_topk_docs_workspace_size(rows, n, k)
+            ws, ws_ptr = _workspace(ws_bytes, self.device)
+            rc = lib.tms_topk_docs(_ptr(scores), rows, n, n, k, _ptr(doc_ids), _ptr(self._lengths), self.n_docs,
+                                   _ptr(vals), _ptr(ids), ws_ptr, ws_bytes, _lib.stream_handle(self.device))
+            _lib.check(rc, "tms_topk_docs")
+            del ws
+        return (vals[0], ids[0]) if single else (vals, ids)
 
     def tokens(self, doc_ids: torch.Tensor | list[int], dtype: torch.dtype = torch.float16
                ) -> tuple[torch.Tensor, torch.Tensor]:
