@@ -274,10 +274,11 @@ class PagedCorpus:
     """A pool of pages with room for n_pages * page_size tokens and max_docs documents.
 
     Documents get ascending ids in the order they are added; a removed document's id is not given
-    out again and scores -inf. All device buffers are allocated here and updated in place, so a
+    out again and scores -inf, and its row of the tables counts towards max_docs until ``compact``
+    drops it and numbers the others anew. All device buffers are allocated here and updated in place, so a
     captured search (``GraphedStep``) sees later additions to the documents it was captured for
     being removed, and never reads memory that was freed; documents added after the capture are not
-    in its output. ``add`` and ``remove`` synchronise with the host; order them against searches on
+    in its output (after a ``compact``, capture it again). ``add`` and ``remove`` synchronise with the host; order them against searches on
     other streams as with any tensor that one stream writes and another reads."""
 
     def __init__(self, d: int, n_pages: int, max_docs: int, page_size: int = 32,
@@ -336,7 +337,8 @@ class PagedCorpus:
         if need > self.n_free:
             raise ValueError(f"{need} pages are needed, {self.n_free} are free")
         if first + n > self.max_docs:
-            raise ValueError(f"no room for {n} documents: {first} of {self.max_docs} are taken")
+            raise ValueError(f"no room for {n} documents: {first} of {self.max_docs} rows are taken, {self._gone()} of "
+                             "them by documents without tokens, which compact() drops")
         ids = torch.arange(first, first + n, device=self.device)
         if n == 0:
             return ids
@@ -388,12 +390,38 @@ class PagedCorpus:
             self._page_ids[used - freed:used] = -1
             self._page_docs[used - freed:used] = -1
             self._lengths[gone] = 0
-            shift = self.page_size - 1
-            self._page_offsets[1:] = torch.cumsum((self._lengths + shift) // self.page_size, 0)
-            self._token_offsets[1:] = torch.cumsum(self._lengths, 0)
+            self._count_offsets()
         self._n_tokens -= int(self._host_lengths[ids].sum())
         self._host_lengths[ids] = 0
         self.n_free += freed
+
+    def _count_offsets(self) -> None:
+        self._page_offsets[1:] = torch.cumsum((self._lengths + self.page_size - 1) // self.page_size, 0)
+        self._token_offsets[1:] = torch.cumsum(self._lengths, 0)
+
+    def _gone(self) -> int:
+        return self.n_docs - int(np.count_nonzero(self._host_lengths[:self.n_docs]))
+
+    def compact(self) -> torch.Tensor:
+        """Drops the rows of documents without tokens (removed, or added empty) and numbers the others
+        anew, in their order: document i becomes the returned (n_docs,) int64 ids' entry i, -1 if it
+        is dropped. No token moves. Ids held elsewhere (an ``IVFIndex``, a captured search) are the old ones."""
+        n, used = self.n_docs, self.n_pages - self.n_free
+        old = np.flatnonzero(self._host_lengths[:n])
+        new = np.full(n, -1, dtype=np.int64)
+        new[old] = np.arange(old.size)
+        with torch.cuda.device(self.device):
+            ids = torch.from_numpy(new).to(self.device)
+            self._page_docs[:used] = ids[self._page_docs[:used].long()].to(torch.int32)
+            kept = self._lengths[torch.from_numpy(old).to(self.device)]
+            self._lengths[:n] = 0
+            self._lengths[:old.size] = kept
+            self._count_offsets()
+        self._host_lengths[:old.size] = self._host_lengths[old]
+        self._host_lengths[old.size:n] = 0
+        self._longest = int(self._host_lengths.max())
+        self.n_docs = old.size
+        return ids
 
     def select(self, doc_ids: torch.Tensor, n_tokens: int | None = None, slots: bool = False) -> PageTables:
         """The tables of the given documents (an id outside the corpus is an empty document).
