@@ -61,3 +61,29 @@ def test_more_documents_than_rows(cuda_device):
     assert c.n_docs == 0 and c.n_free == c.n_pages and sorted(c._free.tolist()) == list(range(c.n_pages))
     assert c.compact().numel() == 0
     assert c.score_queries(Q).shape == (2, 0)
+
+
+def test_tables_hold_the_entries_in_use(cuda_device):
+    """Whether documents are cut over several ranges goes by their mean length, for which a table's capacity
+    stands: the empty part of a large pool does not make short documents long."""
+    from tilemaxsim_b200 import GraphedStep, PagedCorpus, _lib, paged_maxsim
+    c = PagedCorpus(64, n_pages=20000, max_docs=500)
+    Q = _queries(2, 32, 64, 1)
+    assert c.tables.page_ids.numel() == 0 and c.score_queries(Q).shape == (2, 0)
+    c.add(torch.randn(100 * 40, 64, generator=_rng(2)).half().cuda(), [40] * 100)
+    t = c.tables
+    assert t.page_ids.numel() == t.page_docs.numel() == 200 == int(t.page_offsets[-1])
+    size = _lib.load().tms_paged_workspace_size
+    assert size(2, 32, 64, 100, 32, 200) == 0 < size(2, 32, 64, 100, 32, 20000)
+    want = paged_maxsim(Q, c.codes, c.scales, t._replace(page_ids=c._page_ids, page_docs=c._page_docs))
+    assert torch.equal(c.score_queries(Q), want)
+    # a captured call's tables serve what is left of its documents, whatever comes after them
+    step = GraphedStep(c.score_queries, Q)
+    assert torch.equal(step(Q), want.cpu())
+    c.remove(list(range(0, 100, 3)))
+    c.add(torch.randn(300 * 90, 64, generator=_rng(3)).half().cuda(), [90] * 300)
+    got = step(Q)
+    want[:, ::3] = -float("inf")
+    assert torch.equal(got, want.cpu()) and torch.equal(got, c.score_queries(Q)[:, :100].cpu())
+    c.remove(list(range(400)))
+    assert c.tables.page_ids.numel() == 0 and torch.isinf(step(Q)).all() and torch.isinf(c.score_queries(Q)).all()

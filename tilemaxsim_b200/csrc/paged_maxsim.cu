@@ -71,7 +71,9 @@ constexpr float kNegInf = -__builtin_huge_valf();
 // What a range begins with: nothing of its own, a document's first page, or a page inside a document
 // that goes on behind the range.
 constexpr int kRangeEmpty = -3, kRangeClean = -2, kRangeInside = -1;
-constexpr int kSplitTokens = 1024;  // ranges cut documents whose mean length is this or more
+// Ranges cut documents whose mean length is this or more, as far as the host knows it: by the capacity of the
+// tables, which for a selection is a bound (its results do not depend on it; a needless join takes 2 us).
+constexpr int kSplitTokens = 1024;
 constexpr int kSplitDocs = 16;      // and of which there are fewer than this for each range
 constexpr int kMostSms = 160;       // CTAs that the workspace has parts for
 
@@ -919,7 +921,7 @@ Workspace workspace_of(int64_t n_queries, int64_t nq, int64_t d, int64_t n_docs,
     w.packed = static_cast<size_t>(mtiles * 3 * ((d + 127) / 128) * 128) * kRow;
     w.factor = static_cast<size_t>(mtiles) * 128 * sizeof(float);
   }
-  // Mean lengths by the table's capacity, which is all the host knows. Ranges times M tiles are at
+  // Mean lengths by the table's capacity. Ranges times M tiles are at
   // most 4 for each SM (a CTA holds up to four M tiles).
   if (mtiles <= 2 * kMostSms && page_cap * page_size >= n_docs * kSplitTokens && n_docs < kSplitDocs * kMostSms) {
     w.parts = static_cast<size_t>(4 * kMostSms + mtiles) * 8 * 32 * sizeof(float);

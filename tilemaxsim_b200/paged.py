@@ -310,9 +310,11 @@ class PagedCorpus:
 
     @property
     def tables(self) -> PageTables:
-        """The tables of all documents (views of the corpus's own buffers, without slots)."""
-        n = self.n_docs
-        return PageTables(self._page_offsets[:n + 1], self._page_ids, self._page_docs, self._token_offsets[:n + 1], None)
+        """The tables of all documents (views of the corpus's own buffers, without slots). Their capacity
+        is the entries in use: later removals leave fewer, and documents added later are not theirs."""
+        n, used = self.n_docs, self.n_pages - self.n_free
+        return PageTables(self._page_offsets[:n + 1], self._page_ids[:used], self._page_docs[:used],
+                          self._token_offsets[:n + 1], None)
 
     def _pages_of(self, lengths: np.ndarray) -> int:
         return int(((lengths + self.page_size - 1) // self.page_size).sum())
