@@ -304,7 +304,7 @@ TMS_API int tms_page_tables(const int64_t* lengths, int64_t n_lengths, const int
  * tokens rounded to fp32, code = e4m3(y / scale) rounded once to nearest. x, residual: dtype, rows of d
  * elements stride_token apart; padded != 0: document i starts at i * stride_doc and has n_rows
  * rows at most; else its tokens are rows token_offsets[i].. of n_rows. Tokens past n_rows read as
- * zeros. weight: (d) dtype, only with TMS_NORM_RMS, NULL for ones. A page with a NaN or an infinity
+ * zeros. weight: (d) dtype, only with TMS_NORM_RMS, NULL for ones. eps: finite, not negative. A page with a NaN or an infinity
  * among its normalised values gets scale NaN and codes NaN. Buffers 16-byte aligned, strides
  * multiples of 16 bytes. Pages that the tables do not name are left as they were; a page named
  * twice ends up with either content, or a mixture. */

@@ -25,3 +25,37 @@ def test_topk_docs_refusals():
     assert lib.tms_topk_docs_workspace_size(2, 10, 3) == 80
     assert lib.tms_topk_docs_workspace_size(2, 0, 3) == 0
     assert lib.tms_topk_docs_workspace_size(1, 100000, 10) > 800000
+
+
+def _tables(n=2, cap=4):
+    from tilemaxsim_b200 import PageTables
+    return PageTables(torch.zeros(n + 1, dtype=torch.int64), torch.zeros(cap, dtype=torch.int32),
+                      torch.zeros(cap, dtype=torch.int32), torch.zeros(n + 1, dtype=torch.int64), None)
+
+
+@pytest.mark.parametrize("eps", [1e-50, 7e-46, 5e-324, 3.5e38, 1e39, 1e308])
+@pytest.mark.parametrize("norm", ["l2", "rms", "none"])
+def test_eps_outside_fp32(eps, norm):
+    """The kernel takes eps in fp32: one that becomes nothing or infinite there is refused."""
+    from tilemaxsim_b200 import page_write
+    codes, scales = torch.zeros(4, 32, 128, dtype=torch.float8_e4m3fn), torch.zeros(4)
+    with pytest.raises(ValueError, match="eps"):
+        page_write(torch.zeros(8, 128).half(), _tables(), codes, scales, norm=norm, eps=eps)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1.5e-45, 1e-12, 3.4e38])
+def test_eps_inside_fp32(eps):
+    from tilemaxsim_b200 import page_write
+    codes, scales = torch.zeros(4, 32, 128, dtype=torch.float8_e4m3fn), torch.zeros(4)
+    with pytest.raises(ValueError, match="CUDA"):  # the next check
+        page_write(torch.zeros(8, 128).half(), _tables(), codes, scales, eps=eps)
+
+
+def test_c_abi_refuses_an_infinite_eps():
+    from tilemaxsim_b200 import _lib as L
+    lib, nul, p = L.load(), ctypes.c_void_p(0), ctypes.c_void_p(1 << 20)
+    for norm in (0, 1, 2):
+        for eps in (float("inf"), float("nan"), -1.0, -float("inf")):
+            # no documents: refused before there is anything to do, or to read
+            assert lib.tms_page_write(p, 0, 8, 0, 128, 0, nul, nul, norm, ctypes.c_float(eps), 128, 32, p, p, p, p, 0,
+                                      4, p, p, 4, nul) == L.TMS_ERR_INVALID

@@ -1029,7 +1029,7 @@ extern "C" int tms_page_write(const void* x, int dtype, int64_t n_rows, int64_t 
   if (dtype != TMS_F16 && dtype != TMS_BF16 && dtype != TMS_F32) return TMS_ERR_INVALID;
   if (norm != TMS_NORM_NONE && norm != TMS_NORM_L2 && norm != TMS_NORM_RMS) return TMS_ERR_INVALID;
   if (weight && norm != TMS_NORM_RMS) return TMS_ERR_INVALID;
-  if (!(eps >= 0.f)) return TMS_ERR_INVALID;
+  if (!(eps >= 0.f && eps <= 3.4028235e38f)) return TMS_ERR_INVALID;
   if (n_rows < 0 || d <= 0 || n_docs < 0 || page_capacity < 0 || n_pages < 0) return TMS_ERR_INVALID;
   const int shift = page_shift_of(page_size);
   if (shift < 0 || d % 16 != 0 || d > TMS_PAGED_MAX_D) return TMS_ERR_UNSUPPORTED;

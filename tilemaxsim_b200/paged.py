@@ -25,6 +25,7 @@ from . import _lib
 PAGE_SIZES = (16, 32, 64, 128)
 _NORMS = {"none": _lib.TMS_NORM_NONE, "l2": _lib.TMS_NORM_L2, "rms": _lib.TMS_NORM_RMS}
 _EPS = {"none": 0.0, "l2": 1e-12, "rms": 1e-6}
+_FP32_MAX = torch.finfo(torch.float32).max
 
 
 class PageTables(NamedTuple):
@@ -179,8 +180,8 @@ def page_write(x: torch.Tensor, tables: PageTables, codes: torch.Tensor, scales:
     if weight is not None and norm != "rms":
         raise ValueError("weight goes with norm='rms' only")
     eps = _EPS[norm] if eps is None else float(eps)
-    if not 0.0 <= eps < float("inf"):
-        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    if not 0.0 <= eps <= _FP32_MAX or (eps > 0.0 and np.float32(eps) == 0):  # the kernel takes it in fp32
+        raise ValueError(f"eps must be finite and not negative, in fp32 too, got {eps}")
     n_pages, page_size, d = _check_pool(codes, scales)
     n_docs = _check_tables(tables)
     dev = _device(x, codes, scales, tables.page_offsets, tables.page_ids, tables.page_docs, tables.token_offsets,
