@@ -65,7 +65,11 @@ def _page_size(page_size: int) -> int:
 def _ints(t: torch.Tensor, dtype: torch.dtype, name: str) -> torch.Tensor:
     if t.dim() != 1 or (t.dtype != dtype and (t.is_floating_point() or t.is_complex() or t.dtype == torch.bool)):
         raise ValueError(f"{name} must be a 1-D integer tensor, got {t.dtype} {tuple(t.shape)}")
-    return (t if t.dtype == dtype else t.to(dtype)).contiguous()
+    if t.dtype != dtype:
+        if dtype == torch.int32 and t.element_size() >= 4:  # an id that 32 bits do not hold stays one that no pool has
+            t = t.to(torch.int64).clamp(-1, (1 << 31) - 1)
+        t = t.to(dtype)
+    return t.contiguous()
 
 
 def _tables_call(lengths, doc_ids, src_offsets, pages, page_size, n_tokens, with_slots) -> PageTables:
