@@ -59,3 +59,16 @@ def test_c_abi_refuses_an_infinite_eps():
             # no documents: refused before there is anything to do, or to read
             assert lib.tms_page_write(p, 0, 8, 0, 128, 0, nul, nul, norm, ctypes.c_float(eps), 128, 32, p, p, p, p, 0,
                                       4, p, p, 4, nul) == L.TMS_ERR_INVALID
+
+
+@pytest.mark.parametrize("lengths", [
+    [(1 << 63) - 1, (1 << 63) - 1, 2], [(1 << 62)] * 4, [(1 << 63) - 8, 8, 1 << 63], [1 << 40], np.array([(1 << 64) - 3, 3], np.uint64),
+    torch.tensor([(1 << 63) - 1, (1 << 63) - 1, 2]), [(1 << 63) - 1] * 2 + [2] + [0] * 5])
+def test_add_refuses_lengths_whose_sum_wraps(lengths):
+    """Their sum, or the pages they round up to, leaves 64 bits: refused on the host, the corpus as it was."""
+    from tilemaxsim_b200 import PagedCorpus
+    c = PagedCorpus.__new__(PagedCorpus)
+    c.page_size, c.d, c.n_pages, c.max_docs, c.n_docs, c.n_free, c.device = 16, 32, 10, 10, 0, 10, torch.device("cpu")
+    with pytest.raises(ValueError, match="pages are needed|negative|sum to|integers"):
+        c.add(torch.zeros(0, 32).half(), lengths)
+    assert c.n_docs == 0 and c.n_free == 10

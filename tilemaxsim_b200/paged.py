@@ -336,6 +336,8 @@ class PagedCorpus:
         n, n_tok, first = host.size, int(host.sum()), self.n_docs
         if n and host.min() < 0:
             raise ValueError("lengths must not be negative")
+        if n and host.max() > self.n_pages * self.page_size:  # before sums and pages of such lengths can wrap
+            raise ValueError(f"{-(-int(host.max()) // self.page_size)} pages are needed, {self.n_free} are free")
         if x.dim() == 2 and x.shape[0] != n_tok:
             raise ValueError(f"x has {x.shape[0]} tokens, the lengths sum to {n_tok}")
         if x.dim() == 3 and (x.shape[0] != n or host.max(initial=0) > x.shape[1]):
