@@ -87,3 +87,18 @@ def test_tables_hold_the_entries_in_use(cuda_device):
     assert torch.equal(got, want.cpu()) and torch.equal(got, c.score_queries(Q)[:, :100].cpu())
     c.remove(list(range(400)))
     assert c.tables.page_ids.numel() == 0 and torch.isinf(step(Q)).all() and torch.isinf(c.score_queries(Q)).all()
+
+
+def test_captured_search_of_candidates_beside_a_long_document(cuda_device):
+    """Candidates times the longest document is far more than the corpus holds: outside a capture the host
+    looks at their own sum, within one it cannot wait and takes the bound."""
+    from tilemaxsim_b200 import GraphedStep, PagedCorpus
+    c = PagedCorpus(16, n_pages=3000, max_docs=2100, page_size=16)
+    lengths = [1] * 1000 + [20000] + [3] * 700
+    c.add(torch.randn(sum(lengths), 16, generator=_rng(1)).half().cuda(), lengths)
+    Q = _queries(2, 4, 16, 5)
+    pick = [torch.randint(0, 1701, (5000,), generator=_rng(s)).cuda() for s in (2, 3)]
+    step = GraphedStep(lambda q, i: c.search(q, 10, i), Q, pick[0])
+    for ids in (*pick, torch.full((5000,), 1000).cuda()):  # at last the long document, again and again
+        want = c.search(Q, 10, ids)
+        assert all(torch.equal(a, b.cpu()) for a, b in zip(step(Q, ids), want))

@@ -321,6 +321,10 @@ class PagedCorpus:
         return PageTables(self._page_offsets[:n + 1], self._page_ids[:used], self._page_docs[:used],
                           self._token_offsets[:n + 1], None)
 
+    def _capturing(self) -> bool:
+        with _lib.on_device(self.device):
+            return torch.cuda.is_current_stream_capturing()
+
     def _pages_of(self, lengths: np.ndarray) -> int:
         return int(((lengths + self.page_size - 1) // self.page_size).sum())
 
@@ -435,11 +439,12 @@ class PagedCorpus:
     def select(self, doc_ids: torch.Tensor, n_tokens: int | None = None, slots: bool = False) -> PageTables:
         """The tables of the given documents (an id outside the corpus is an empty document).
         n_tokens bounds their tokens. By default it is the longest document's length for each, and
-        where that is far more than the corpus holds, their own sum, for which the host waits."""
+        where that is far more than the corpus holds, their own sum, for which the host waits (but
+        not in a capture, whose replays bring other documents: the bound stays)."""
         doc_ids = _ints(doc_ids, torch.int64, "doc_ids")
         if n_tokens is None:
             n_tokens = doc_ids.numel() * self._longest
-            if n_tokens > max(4 * self._n_tokens, 1 << 24):
+            if n_tokens > max(4 * self._n_tokens, 1 << 24) and not self._capturing():
                 inside = (doc_ids >= 0) & (doc_ids < self.n_docs)
                 n_tokens = int(self._lengths[doc_ids.clamp(0, self.max_docs - 1)][inside].sum())
         n = self.n_docs
