@@ -32,3 +32,66 @@ def test_page_ids_of_64_bits_do_not_wrap(bad, cuda_device):
     lengths, offsets = torch.tensor([16, 16, 16], device=cuda_device), torch.arange(4, device=cuda_device)
     s = select_page_tables(lengths, 16, offsets, ids, torch.tensor([1, 2], device=cuda_device), 32)
     assert not 0 <= s.page_ids[0].item() < 1 << 27 and s.page_ids[1].item() == 1
+
+
+def _four_squares(n):
+    """Four whole numbers whose squares sum to n."""
+    for a in range(int(n ** 0.5), -1, -1):
+        for b in range(int(max(n - a * a, 0) ** 0.5), -1, -1):
+            rest = n - a * a - b * b
+            for c in range(int(rest ** 0.5), int((rest / 2) ** 0.5) - 1, -1):
+                d = round((rest - c * c) ** 0.5)
+                if c * c + d * d == rest:
+                    return [a, b, c, d]
+    raise AssertionError(n)
+
+
+def _row_of_ties(d, rng, norm):
+    """Whole numbers whose squares sum to norm^2 = (3 * 2^k)^2, the largest 7 norm / 16, and sixteen of those
+    that lie exactly between two codes once divided by the norm and by the scale that the largest gives (2^-10)."""
+    top = 7 * norm // 16
+    ties = [3 * m * norm // 768 for m in list(range(17, 32, 2)) + list(range(34, 64, 4)) + list(range(68, 84, 8))]
+    row = [top] + rng.choice(ties, 16).tolist()
+    while (rest := norm * norm - sum(v * v for v in row)) > 4 * top * top:
+        row.append(top)
+    if rest < 0 or len(row) > d - 4:
+        return None
+    row += _four_squares(rest)
+    row += [0] * (d - len(row))
+    return None if max(row) > top else [v * s for v, s in zip(row, rng.choice([-1, 1], d))]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("norm,residual,weight", [("l2", False, None), ("l2", True, None), ("rms", False, None), ("rms", True, 3.0),
+                                                   ("rms", False, 0.5)])
+@pytest.mark.parametrize("page,d", [(16, 64), (32, 128), (128, 64), (64, 256)])
+def test_write_exact_ties_of_normalised_values(page, d, norm, residual, weight, dtype, cuda_device):
+    """Norms and scales that are exact: what lies between two codes goes to the even one, decided by the
+    norm's quotient itself, not by a factor that comes near it."""
+    from tilemaxsim_b200 import page_tables, page_write
+    rng = np.random.default_rng(page + d)
+    rows = []
+    while len(rows) < page:
+        r = _row_of_ties(d, rng, 768)
+        rows += [r] if r else []
+    h = np.array(rows, dtype=np.float64)
+    assert ((h * h).sum(1) == 768.0 ** 2).all()
+    res = rng.integers(-64, 65, h.shape) if residual else None
+    x = torch.from_numpy(h if res is None else h - res).to(dtype)
+    assert (x.double().numpy() + (0 if res is None else res) == h).all()
+    w = None if weight is None else torch.full((d,), weight).to(dtype)
+    codes, scales = _pool(1, page, d)
+    t = page_tables(torch.tensor([page], device=cuda_device), page, torch.zeros(1, dtype=torch.int32, device=cuda_device), page)
+    page_write(x.cuda(), t, codes, scales, residual=None if res is None else torch.from_numpy(res).to(dtype).cuda(),
+               weight=None if w is None else w.cuda(), norm=norm, eps=0.0)
+    n = 768.0 if norm == "l2" else np.sqrt(768.0 ** 2 / d)
+    y = h / n * (weight or 1.0)
+    scale = float(np.float32(np.abs(y).max() / 448))
+    assert scales.item() == scale
+    v = h * (weight or 1.0) / (n * scale)
+    if scale == np.abs(y).max() / 448:  # where the scale is not rounded there are ties
+        step = 2 * R.half_step(v)
+        assert (np.abs(v / step % 1 - 0.5) == 0).mean() >= 16 / d
+    step = 2 * R.half_step(v)
+    want = np.clip(np.round(v / step) * step, -448, 448)  # np.round: ties to even
+    np.testing.assert_array_equal(codes[0].cpu().double().numpy(), want)

@@ -412,7 +412,8 @@ struct Eight {
 // comes within 2^-19 of the page's can set the scale: they (one, as a rule) are summed again in
 // fp64. A code is that of t = h * w * factor / scale: where t * (1 - 2^-20) and t * (1 + 2^-20)
 // round to the same one, fp32 is sure of it; the others (about one of 4,000 groups of eight
-// elements) are done again in fp64, with a division. Where nothing is normalised, added or weighted,
+// elements) are done again in fp64, with its root and a division: whole numbers of a rational length
+// have exact ties, which a factor 2^-42 off would break to one side. Where nothing is normalised, added or weighted,
 // ties are common and exact, and one fp32 division with its remainder decides them (5,000 documents:
 // 196 us against 247 with fp64's). Pages that hold a magnitude or a sum of squares outside [1e-30,
 // 1e30], zeros apart, go through fp64 altogether; NaN and infinities are found there.
@@ -480,10 +481,10 @@ struct PageRows {
 };
 
 // A row in fp64, by the lanes that hold it: its eight elements a lane (times the weights), its
-// largest magnitude before the factor, and its factor: from fp32's one by a Newton step, which
-// squares its 2^-21, or, where `full`, by fp64's own root and quotient.
+// largest magnitude, and what both are to be divided by: fp64's own root, where `full`, or the inverse of a
+// factor that a Newton step, which squares fp32's 2^-21, gives (`factor`; cheaper, but off a tie).
 struct ExactRow {
-  double h[8], factor, top;
+  double h[8], factor, norm, top;
   bool bad;
 };
 template <typename T, bool SUM, bool WEIGHT, bool STAGED, int D>
@@ -519,7 +520,7 @@ __device__ __forceinline__ void exact_row(const PageRows<T, SUM, WEIGHT, STAGED,
     for (int m = rows.group >> 1; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
     o.top = top;
   }
-  o.factor = 1.0;
+  o.factor = o.norm = 1.0;
   o.bad = false;
   if (!full) {
     const double f = near, v = a.norm == TMS_NORM_RMS ? s * (1.0 / rows.d) + a.eps : s;
@@ -528,11 +529,11 @@ __device__ __forceinline__ void exact_row(const PageRows<T, SUM, WEIGHT, STAGED,
   }
   if (a.norm == TMS_NORM_L2) {
     const double n = sqrt(s);
-    o.factor = 1.0 / (n > a.eps ? n : static_cast<double>(a.eps));
+    o.norm = n > a.eps ? n : static_cast<double>(a.eps);
   } else if (a.norm == TMS_NORM_RMS) {
-    o.factor = 1.0 / sqrt(s / rows.d + a.eps);
+    o.norm = sqrt(s / rows.d + a.eps);
   }
-  o.bad = !(finite(s) && finite(o.top * o.factor));
+  o.bad = !(finite(s) && finite(o.top / o.norm));
 }
 
 template <typename T, bool SUM, bool WEIGHT, bool STAGED, int D, int kWriteThreads>
@@ -727,7 +728,7 @@ page_write_kernel(const WriteArgs a, int lanes) {
         ExactRow exact;
         exact_row(rows, e, r, row_factor[r], odd, exact);
         bad |= exact.bad;
-        const double y = exact.top * exact.factor;
+        const double y = odd ? exact.top / exact.norm : exact.top * exact.factor;
         if (y > best) best = y;
       }
     }
@@ -794,12 +795,13 @@ page_write_kernel(const WriteArgs a, int lanes) {
         const int row = r0 + i * step;
         const int src = row < e.count ? row : e.count - 1;
         ExactRow exact;
-        exact_row(rows, e, src, row_factor[src], !plain, exact);
+        exact_row(rows, e, src, 0.f, true, exact);
         if (!(unsure >> i & 1u) || row >= page || !in_row) continue;
         uint32_t word[2] = {0, 0};
+        const double by = exact.norm * scale;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const uint32_t code = bad ? 0x7fu : scale > 0.f ? e4m3_of_double(exact.h[j] * exact.factor / scale) : 0u;
+          const uint32_t code = bad ? 0x7fu : scale > 0.f ? e4m3_of_double(exact.h[j] / by) : 0u;
           word[j >> 2] |= code << (8 * (j & 3));
         }
         *reinterpret_cast<uint2*>(out + row * d) = make_uint2(word[0], word[1]);
