@@ -95,3 +95,34 @@ def test_write_exact_ties_of_normalised_values(page, d, norm, residual, weight, 
     step = 2 * R.half_step(v)
     want = np.clip(np.round(v / step) * step, -448, 448)  # np.round: ties to even
     np.testing.assert_array_equal(codes[0].cpu().double().numpy(), want)
+
+
+@pytest.mark.parametrize("small,weight,eps", [(1e-26, 1e-24, e) for e in (0.0, 1e-38, 1e-30, 1e-20, 1e-7)]
+                         + [(1e-24, 1e-22, e) for e in (1e-42, 1e-40, 1e-38, 1e-37, 1e-30)])
+@pytest.mark.parametrize("d,page", [(16, 16), (128, 32)])
+def test_write_products_with_weights_below_fp32(d, page, small, weight, eps, cuda_device):
+    """h * weight and h^2 vanish in fp32 where their quotient by the root does not: fp64 decides. Beside
+    them rows of zeros, in a page of their own and in one with others."""
+    from tilemaxsim_b200 import page_tables, page_write
+    g = _rng(d)
+    x = torch.randn(2 * page + 3, d, generator=g) * small
+    x[1] = 0
+    x[page:2 * page] = 0
+    w = (1 + 0.1 * torch.randn(d, generator=g)) * weight
+    lengths = [page, page, 3]
+    t = page_tables(torch.tensor(lengths, device=cuda_device), page, torch.arange(3, dtype=torch.int32, device=cuda_device), len(x))
+    codes, scales = _pool(3, page, d)
+    page_write(x.cuda(), t, codes, scales, norm="rms", weight=w.cuda(), eps=eps)
+    # without an eps a row of zeros is not a number
+    with np.errstate(invalid="ignore"):
+        y = R.normalise(x.double().numpy(), None, w.double().numpy(), "rms", float(np.float32(eps)))
+    for i, rows in enumerate(np.split(y, [page, 2 * page])):
+        s = scales[i].item()
+        if np.isnan(rows).any():
+            assert np.isnan(s)
+            continue
+        want = np.abs(rows).max() / 448
+        assert abs(s - want) <= max(want * 2.0 ** -24 * 1.0001, 2.0 ** -150)
+        if s > 0:
+            v = rows / s
+            assert (np.abs(codes[i, :len(rows)].cpu().double().numpy() - np.clip(v, -448, 448)) <= R.half_step(np.clip(v, -448, 448)) * (1 + 1e-9)).all()
