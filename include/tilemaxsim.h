@@ -330,7 +330,7 @@ TMS_API size_t tms_paged_workspace_size(int64_t n_queries, int64_t nq, int64_t d
  * d) fp16 or bf16, 16-byte aligned. n_pages * page_size < 2^31,
  * page_capacity * max(page_size / 32, 1) < 2^30 and n_queries * ceil(nq / 32) < 2^24. A query row
  * with a NaN or an infinity makes its query's scores NaN. Q is read through a power-of-two scaling
- * of each row that keeps an element to 2^-17 of its row's largest magnitude or better. */
+ * of each row that keeps an element to 2^-21 of its row's largest magnitude or better. */
 TMS_API int tms_paged_maxsim(const void* Q, int q_dtype, int64_t n_queries, int64_t nq, int64_t d,
                              const void* codes, const float* scales, int64_t n_pages,
                              int64_t page_size, const int64_t* page_offsets,

@@ -126,3 +126,38 @@ def test_write_products_with_weights_below_fp32(d, page, small, weight, eps, cud
         if s > 0:
             v = rows / s
             assert (np.abs(codes[i, :len(rows)].cpu().double().numpy() - np.clip(v, -448, 448)) <= R.half_step(np.clip(v, -448, 448)) * (1 + 1e-9)).all()
+
+
+def _wide_rows(n, d, seed):
+    """Rows whose elements lie far apart: one outlier beside a normal distribution, magnitudes over many powers of
+    two, one element alone, and ordinary ones."""
+    g = _rng(seed)
+    q = torch.randn(n, d, generator=g)
+    q[0::4, d // 3] = 64.0
+    wide = torch.exp2(-20 * torch.rand(n, d, generator=g)) * q.sign()
+    q[1::4] = wide[1::4]
+    q[2::4] *= 0.01
+    q[2::4, d - 1] = -3.0
+    return q
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bq,nq", [(1, 1), (1, 32), (2, 5), (1, 64), (3, 20), (20, 32), (5, 1)])
+@pytest.mark.parametrize("page,d", [(16, 64), (32, 64), (32, 128), (16, 128), (32, 96), (64, 256), (16, 144)])
+def test_scores_find_every_element_of_a_query(page, d, bq, nq, dtype, cuda_device):
+    """A document for each dimension, whose token is nothing elsewhere: its score is that element of the
+    query's rows. The row's largest magnitude being 128 or more of a unit, an element is held to 2^-14 of
+    that unit, 2^-21 of the largest magnitude, and its terms' products and the row's sums are fp32."""
+    from tilemaxsim_b200 import page_tables, page_write, paged_maxsim
+    codes, scales = _pool(d, page, d)
+    t = page_tables(torch.ones(d, dtype=torch.int64, device=cuda_device), page,
+                    torch.randperm(d, generator=_rng(1)).to(torch.int32).to(cuda_device), d)
+    page_write((448 * torch.eye(d)).half().cuda(), t, codes, scales, norm="none")
+    assert (scales == 1).all()
+    Q = _wide_rows(bq * nq, d, d + bq).view(bq, nq, d).to(dtype)
+    got = paged_maxsim(Q.cuda(), codes, scales, t).cpu().double() / 448
+    q = Q.double()
+    big = q.abs().amax(-1, keepdim=True)
+    bound = (big * 2.0 ** -21 + q.abs() * (nq + 4) * 2.0 ** -23).sum(1)
+    off = (got - q.sum(1)).abs()
+    assert (off <= bound).all(), (off / bound).max()

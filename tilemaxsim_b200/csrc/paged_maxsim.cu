@@ -7,11 +7,13 @@
 //
 // The codes go to the tensor cores as they are stored (tcgen05 kind::f8f6f4, fp32 accumulators).
 // A 16-bit query element does not fit e4m3's four significant bits, so each query row is scaled by
-// a power of two (its largest magnitude lands in [128, 256)) and split into e4m3 terms, each the
-// rounding of what the terms before it left: two terms hold bf16's eight bits, three hold fp16's
-// eleven. The terms are laid side by side along K against the same tokens, so one accumulator
-// holds the whole product. What is lost lies under e4m3's smallest step: an element below 2^-9
-// (bf16) or 2^-6 (fp16) of its row's largest is off by at most 2^-17 of that largest.
+// a power of two (its largest magnitude lands in [128, 256)) and split into terms, each the rounding
+// of what the terms before it left, e4m3 ones and an e5m2 one last: two terms hold bf16's eight bits,
+// three hold fp16's eleven, the last three of them at most in the last term. The terms are laid side by
+// side along K against the same tokens, so one accumulator holds the whole product. What is lost lies
+// under e5m2's three bits of what e4m3's smallest step, 2^-9, leaves: an element below 2^-13 (bf16) or
+// 2^-10 (fp16) of its row's largest is off by at most 2^-21 of that largest. (With an e4m3 term last it
+// was 2^-17 of it, at the same speed.)
 //
 // Work split. The table entries (pages) are cut into ranges at document boundaries, one a CTA, and
 // each range evenly into S streams. A tile is 256 token columns: W = 256 / S of each stream's next
@@ -190,7 +192,7 @@ __device__ __forceinline__ uint32_t elect_one() {
       : "=r"(r));
   return r;
 }
-// D(tmem) (+)= A * B^T, both K-major e4m3 in shared memory, fp32 accumulation, issued by the lane
+// D(tmem) (+)= A * B^T, both K-major 8-bit in shared memory, fp32 accumulation, issued by the lane
 // whose `leader` is set. The whole warp runs the loop around it: the descriptors then stay in
 // uniform registers (64 queries, 4k documents: 423 us under "lane == 0", 324 us so at the time).
 __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
@@ -275,7 +277,7 @@ __device__ __forceinline__ int64_t clamp_entry(const PagedArgs& a, int64_t v) {
   return v < 0 ? 0 : v > a.page_cap ? a.page_cap : v;
 }
 
-// Rows [r0, r0 + kPackRows) of an M tile (32 * nc rows) as e4m3 terms in the 128-byte-swizzle layout
+// Rows [r0, r0 + kPackRows) of an M tile (32 * nc rows) as e4m3 and e5m2 terms in the 128-byte-swizzle layout
 // (16-byte unit u of row r at u ^ (r % 8); tiles [term][K chunk][row]) at `tile`, and for each row
 // the power of two to undo at `factor`. One warp, a lane four elements of each 128-byte chunk.
 constexpr int kPackRows = 4;
@@ -344,11 +346,16 @@ __device__ __forceinline__ void pack_rows(const PagedArgs& a, int nc, int m, int
         uint32_t word = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const __nv_fp8x2_storage_t two =
-              __nv_cvt_float2_to_fp8x2(make_float2(rest[2 * h], rest[2 * h + 1]), __NV_SATFINITE, __NV_E4M3);
-          const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
-          rest[2 * h] -= back.x;
-          rest[2 * h + 1] -= back.y;
+          const float2 now = make_float2(rest[2 * h], rest[2 * h + 1]);
+          __nv_fp8x2_storage_t two;
+          if (t == a.terms - 1) {
+            two = __nv_cvt_float2_to_fp8x2(now, __NV_SATFINITE, __NV_E5M2);
+          } else {
+            two = __nv_cvt_float2_to_fp8x2(now, __NV_SATFINITE, __NV_E4M3);
+            const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+            rest[2 * h] -= back.x;
+            rest[2 * h + 1] -= back.y;
+          }
           word |= static_cast<uint32_t>(two) << (16 * h);
         }
         *reinterpret_cast<uint32_t*>(at) = word;
@@ -563,6 +570,7 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
     if (warp == 1) {
       // ---------------------------------------------------------------- MMA issue
       constexpr uint32_t idesc = make_idesc(32 * NC, PAIR ? kTile / 2 : kTile, 0);  // e4m3 operands, fp32 accumulator
+      constexpr uint32_t idesc_last = idesc | 1u << 7;  // the last term: A is e5m2
       const uint32_t leader = elect_one();
       const uint64_t desc0 = sw128_kmajor_desc(0);
       auto desc = [&](uint32_t lo) { return desc0 & ~0xffffffffull | lo; };  // steps stay in the low word
@@ -598,12 +606,12 @@ paged_mma_kernel(const __grid_constant__ CUtensorMap codes_map, const __grid_con
             auto step = [&](auto three, uint32_t to, uint32_t at, uint32_t bt, uint32_t acc) {  // 32 elements of K
               if constexpr (NC == 4) {
                 mma_f8(to, desc(at), desc(bt), idesc, acc, leader);
-                mma_f8(to, desc(at + term_step), desc(bt), idesc, 1, leader);
-                if constexpr (three.value) mma_f8(to, desc(at + 2 * term_step), desc(bt), idesc, 1, leader);
+                if constexpr (three.value) mma_f8(to, desc(at + term_step), desc(bt), idesc, 1, leader);
+                mma_f8(to, desc(at + (three.value ? 2 : 1) * term_step), desc(bt), idesc_last, 1, leader);
               } else {
                 mma_f8_ws<0>(to, desc(at), desc(bt), idesc, acc, leader);
                 if constexpr (three.value) mma_f8_ws<1>(to, desc(at + term_step), desc(bt), idesc, 1, leader);
-                mma_f8_ws<2>(to, desc(at + (three.value ? 2 : 1) * term_step), desc(bt), idesc, 1, leader);
+                mma_f8_ws<2>(to, desc(at + (three.value ? 2 : 1) * term_step), desc(bt), idesc_last, 1, leader);
               }
             };
             // The issuing warp's own instructions count: one warp alone takes several clocks for each.
