@@ -102,3 +102,33 @@ def test_captured_search_of_candidates_beside_a_long_document(cuda_device):
     for ids in (*pick, torch.full((5000,), 1000).cuda()):  # at last the long document, again and again
         want = c.search(Q, 10, ids)
         assert all(torch.equal(a, b.cpu()) for a, b in zip(step(Q, ids), want))
+
+
+@pytest.mark.parametrize("bq,nq,d,page", [(1, 32, 128, 32), (2, 32, 64, 16), (4, 20, 128, 64), (20, 32, 128, 32), (3, 77, 256, 16)])
+def test_alone_and_among_others(bq, nq, d, page, cuda_device):
+    """A query by itself and in a batch, a document by itself, among candidates and in a corpus of many
+    steps: every score is within the bound of 64 bits' over the tokens that the pages hold."""
+    import paged_ref as R
+    from tilemaxsim_b200 import PagedCorpus
+    lengths = torch.randint(0, 130, (8000,), generator=_rng(d)).tolist()
+    c = PagedCorpus(d, n_pages=sum(-(-n // page) for n in lengths), max_docs=8000, page_size=page)
+    c.add(torch.randn(sum(lengths), d, generator=_rng(1)).half().cuda(), lengths)
+    Q = _queries(bq, nq, d, 2, torch.bfloat16)
+    pick = [i for i in torch.randperm(8000, generator=_rng(3))[:60].tolist() if lengths[i]][:40]
+    tok, off = c.tokens(pick, torch.float32)
+    docs = [v.cpu().double().numpy() for v in tok.split((off[1:] - off[:-1]).tolist())]
+    q = Q.cpu().double().numpy()
+    want, bound = R.scores(q, docs), R.score_bound(q, docs)
+    ids = torch.tensor(pick, device=cuda_device)
+
+    def check(got, w, b):
+        assert (abs(got.cpu().double().numpy() - w) <= b).all()
+
+    check(c.score_queries(Q)[:, ids], want, bound)
+    check(c.score_queries(Q, ids), want, bound)
+    for i in range(0, bq, 3):
+        check(c.score_queries(Q[i])[ids], want[i], bound[i])
+        check(c.score_queries(Q[i:i + 1], ids), want[i:i + 1], bound[i:i + 1])
+    for j in range(0, len(pick), 4):
+        check(c.score_queries(Q, ids[j:j + 1]), want[:, j:j + 1], bound[:, j:j + 1])
+        check(c.score_queries(Q[-1], ids[j:j + 1]), want[-1, j:j + 1], bound[-1, j:j + 1])
