@@ -300,14 +300,15 @@ TMS_API int tms_page_tables(const int64_t* lengths, int64_t n_lengths, const int
                             void* workspace, size_t workspace_bytes, void* stream);
 
 /* Writes the documents of the tables (as tms_page_tables makes them) into their pages: token h =
- * x (+ residual), normalised as `norm` says (fp64 sums), scale = max |y| / 448 over the page's
- * tokens rounded to fp32, code = e4m3(y / scale) rounded once to nearest. x, residual: dtype, rows of d
+ * x (+ residual), normalised as `norm` says, scale = max |y| / 448 over the page's tokens rounded to
+ * fp32, code = e4m3(y / scale) rounded once to nearest, ties to even: sums run in fp32, and what they
+ * leave open (the scale, values beside a midpoint) is decided in fp64. x, residual: dtype, rows of d
  * elements stride_token apart; padded != 0: document i starts at i * stride_doc and has n_rows
  * rows at most; else its tokens are rows token_offsets[i].. of n_rows. Tokens past n_rows read as
- * zeros. weight: (d) dtype, only with TMS_NORM_RMS, NULL for ones. eps: finite, not negative. A page with a NaN or an infinity
- * among its normalised values gets scale NaN and codes NaN. Buffers 16-byte aligned, strides
- * multiples of 16 bytes. Pages that the tables do not name are left as they were; a page named
- * twice ends up with either content, or a mixture. */
+ * zeros. weight: (d) dtype, only with TMS_NORM_RMS, NULL for ones. eps: finite, not negative. A page
+ * with a NaN or an infinity among its normalised values gets scale NaN and codes NaN. Buffers 16-byte
+ * aligned, strides multiples of 16 bytes. Pages that the tables do not name are left as they were; a
+ * page named twice ends up with either content, or a mixture. */
 TMS_API int tms_page_write(const void* x, int dtype, int64_t n_rows, int64_t stride_doc,
                            int64_t stride_token, int padded, const void* residual,
                            const void* weight, int norm, float eps, int64_t d, int64_t page_size,

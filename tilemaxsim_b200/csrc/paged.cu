@@ -157,8 +157,9 @@ __device__ __forceinline__ int64_t owner_of(const int64_t* page_offsets, int64_t
   return lo;
 }
 
-// 400,000 documents (72.8M slots, 582 MB) take 125 us here and 12 us for their offsets; a plain fill
-// of the slots takes 81 us. A slot at a time with its own bounds checks took 219 us.
+// 400,000 documents (72.8M slots, 582 MB) take 126 us here and 12 us for their offsets; a plain fill
+// of the slots takes 81 us. Issue slots are 58% busy; the rest is waits for the entries' loads and for
+// shuffles. A slot at a time with its own bounds checks took 219 us.
 //
 // Page ids, owners and slots of the 32 table entries from k0 on, by one warp: a lane for each entry
 // (`doc` owns it, where it lies below the total), then the entries' slots one after the other. The
@@ -404,8 +405,8 @@ struct Eight {
 
 // One page at a time a CTA of one, two or four warps, the next page on its way into shared memory (cp.async)
 // meanwhile; a group of 2 to 32 lanes takes a row, eight elements a lane. The input is read from
-// memory once and the codes are written once, which bounds the kernel. Pages of more than
-// kStageBytes of input are read twice instead, the second time from the caches.
+// memory once and the codes are written once. Pages of more than kStageBytes of input are read twice
+// instead, the second time from the caches (3.64M tokens of 128 bf16 values in pages of 128: 825 us).
 //
 // The scale is the fp32 rounding, and every code the e4m3 rounding, of what 64 bits give, at little
 // more than fp32's cost. fp32 gives every row's factor to 2^-21. Only rows whose largest magnitude
@@ -415,22 +416,23 @@ struct Eight {
 // elements) are done again in fp64, with its root and a division: whole numbers of a rational length
 // have exact ties, which a factor 2^-42 off would break to one side. Where nothing is normalised, added or weighted,
 // ties are common and exact, and one fp32 division with its remainder decides them (5,000 documents:
-// 196 us against 247 with fp64's). Pages that hold a magnitude or a sum of squares outside [1e-30,
+// 164 us; fp64's took a quarter more). Pages that hold a magnitude or a sum of squares outside [1e-30,
 // 1e30], zeros apart, go through fp64 altogether; NaN and infinities are found there.
 //
-// 20,000 documents (3.6M tokens, 128 bf16 values, unit length) take 456 us, 3.1 TB/s: issue slots (62%
-// busy), not memory, bound it, which is why the width is a constant of the kernel where it is 128 (D).
-// Without that they take 546 us, and 1,600 pages with a residual 17 us against 14.9; the page size as
-// a constant too would give 2% more. Before, rows held in registers took 770 us (few warps fit), all
+// 20,000 documents (3.6M tokens, 128 bf16 values, unit length) take 452 us, 3.1 TB/s. Neither memory nor
+// issue slots (62% busy) are full: with 21 warps an SM, a warp waits for its CTA's barriers, for fixed
+// latencies and for shared memory, in about equal parts. Fewer instructions help all the same: with the
+// width as a constant of the kernel where it is 128 (D) that took a sixth less, and 1,600 pages with a
+// residual 14.9 us against 17; the page size as a constant too would give 2% more. Before, rows held in registers took 770 us (few warps fit), all
 // sums in fp64 600-820, sixteen elements a lane 546, fp64 roots for the rows that set the scale 830.
 __device__ __forceinline__ double max_keep_nan(double x, double y) { return y <= x || x != x ? x : y; }
 __device__ __forceinline__ bool usual(float v) { return v >= 1e-30f && v <= 1e30f; }
 
 // Threads of a CTA: 32 where a page's input is 4 KB at most, 64 up to 8 KB, else 128: as many CTAs as
 // shared memory has stages for then have warps enough, and few warps a page wait for one another
-// little. 3.64M tokens of bf16: d = 64 294 us with 32 threads, 413 with 64; pages of 16 478 and 702;
-// pages of 32 523-610 with 32, 456 with 64, 555 with 128. 1,024 documents with a residual (16 KB a page):
-// 51 us with 64, 43 with 128.
+// little. 3.64M tokens of bf16: d = 64 288 us with 32 threads, 342 with 64; pages of 16 468 and 572;
+// pages of 32 515 with 32, 452 with 64, 548 with 128; pages of 64 538 with 64, 456 with 128; d = 256
+// 1,232 and 1,030. 1,024 documents with a residual (16 KB a page): 52 us with 64, 45 with 128.
 constexpr int write_threads(int input) { return input <= 4096 ? 32 : input <= 8192 ? 64 : 128; }
 constexpr int kStaticBytes = 2048;       // a CTA's other shared memory, at most
 constexpr int kStageBytes = 24 * 1024;  // most input of a page (x and residual) that is staged
@@ -875,8 +877,8 @@ struct ReadArgs {
 // in fp32, then one rounding to the output type. A group of lanes takes a row, sixteen elements a
 // lane (one 16-byte load), and a thread ROWS rows, whose loads are all in flight before the first
 // store: what bounds it is memory. The output is written past the caches' working set. 3.6M rows of
-// 128 to bf16 take 253 us with two rows and 235 us with four (5.8 TB/s), 182 thousand to fp16 take
-// 12.6 and 14.9 us: four where that makes 32 CTAs an SM and more, two below.
+// 128 to bf16 take 299 us with two rows and 266 us with four (5.3 TB/s), 182 thousand to fp16 15.5 us
+// with either: four where that makes 32 CTAs an SM and more, two, which start sooner, below.
 
 template <typename T>
 __device__ __forceinline__ uint32_t two_as(float x, float y) {

@@ -31,15 +31,15 @@
 // halves the rows that the TMA brings and the stage's bytes: the MMAs take N = 128 rows twice, their first
 // 64 bytes and their second, into the two halves of the columns.
 //
-// What bounds it. One query over 100k documents (18.2M tokens, 2.53 GB of pages): memory, 405 us, 6.2
-// TB/s. 64 queries over 4,000 documents: the tensor cores, 251 us, 1,520 TFLOP/s of the query's own
-// products, which the two terms double; after a second of it the power cap, 285 us. 5 queries of 77 rows
-// at d = 256 in fp16 (three terms): the tensor cores, 222 us, 240 under the cap. Few chunks of narrow
-// tokens: the instructions that a warp's own loop takes for a tile, where each waits for the one before.
-// 18.2M tokens of d = 64: 260 us, the MMA warp (397 us with loops and 64-bit descriptors around its 8
-// MMAs and one wait after the other). d = 64, pages of 16, 5.1M tokens, 3 queries: 111 us, the epilogue
-// and the 16 boxes a tile (139 us at first). Copying the pages by cp.async in place of the TMA: 154 us with four
-// warps, 181-228 with two.
+// What bounds it (in a few passes, and in passes without end, which run into the power cap and other inputs).
+// One query over 100k documents (18.2M tokens, 2.53 GB of pages): memory, 402 and 443 us, 6.3 and 5.7
+// TB/s. 64 queries over 4,000 documents: the tensor cores, 252 and 298 us, 1,510 and 1,280 TFLOP/s of the
+// query's own products, which the two terms double. 5 queries of 77 rows at d = 256 in fp16 (three
+// terms): the tensor cores, 221 and 259 us. Few chunks of narrow tokens: the instructions that a warp's
+// own loop takes for a tile, where each waits for the one before. 18.2M tokens of d = 64: 265 us, the
+// MMA warp (397 us with loops and 64-bit descriptors around its 8 MMAs and one wait after the other).
+// d = 64, pages of 16, 5.1M tokens, 3 queries: 123 and 136 us, the epilogue, the MMA warp and the 16 boxes
+// a tile. Copying the pages by cp.async in place of the TMA: 154 us with four warps, 181-228 with two.
 //
 // Warp roles (320 threads, one CTA an SM): warp 0 loads pages by TMA (a lane for each box of up to
 // 32 rows), warp 1 owns TMEM and issues the MMAs, warps 2-9 are the epilogue. A document that ends

@@ -239,7 +239,8 @@ def page_read(codes: torch.Tensor, scales: torch.Tensor, slots: torch.Tensor,
 def paged_maxsim(Qb: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, tables: PageTables) -> torch.Tensor:
     """MaxSim of every query against every document of the tables, straight from the pages.
 
-    Qb: (B_q, Nq, d) or (Nq, d), fp16 or bf16 (fp32 is rounded to fp16). Returns fp32 (B_q, n_docs),
+    Qb: (B_q, Nq, d) or (Nq, d), fp16 or bf16 (fp32 is rounded to fp16, where magnitudes of 65,520 and
+    more are infinite and make the query's scores NaN: give such queries in bf16). Returns fp32 (B_q, n_docs),
     or (n_docs,) for a single 2-D query. A document without pages scores -inf, one with a NaN among
     its pages NaN."""
     lib = _lib.load()
