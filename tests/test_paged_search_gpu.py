@@ -167,3 +167,20 @@ def test_lowest_scores_keep_their_order(cuda_device):
     vals, ids = c.search(torch.full((1, 4, 16), 1e30, dtype=torch.bfloat16, device=cuda_device), 5,
                          torch.tensor([0, 1, 2, 3, 4], device=cuda_device))
     assert ids.tolist() == [[2, 4, 1, 3, 0]] and vals[0, 3].isnan()
+
+
+def test_ivf_returns_documents_that_score_minus_infinity(cuda_device):
+    """Only documents without tokens are padding, not those whose scores overflow."""
+    from tilemaxsim_b200 import IVFIndex, PagedCorpus
+    c = PagedCorpus(16, n_pages=8, max_docs=8, page_size=16)
+    x = torch.full((5, 16), 1e30)
+    x[1:4] *= -1
+    c.add(x.cuda(), [1] * 5, norm="none")
+    index = IVFIndex(torch.ones(1, 16, device=cuda_device), torch.zeros(5, dtype=torch.int64, device=cuda_device),
+                     torch.arange(6, device=cuda_device))
+    Q = torch.full((2, 4, 16), 1e30, dtype=torch.bfloat16, device=cuda_device)
+    c.remove([2, 4])
+    for k in (3, 5):
+        vals, ids = index.search(Q, c, k, nprobe=1)
+        assert ids.tolist() == [[0, 1, 3, -1, -1][:k]] * 2
+        assert vals[:, 0].tolist() == [float("inf")] * 2 and (vals[:, 1:] == float("-inf")).all()

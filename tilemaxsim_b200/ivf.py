@@ -111,7 +111,11 @@ class IVFIndex:
         if n_cand == 0 or Bq == 0:
             return vals, ids
         with torch.cuda.device(self.device):
-            scores = D_tokens.score_queries(Qb, cand) if paged else self._score_gathered(Qb, D_tokens, cand)
+            if paged:
+                scores = D_tokens.score_queries(Qb, cand)
+                scores.masked_fill_(D_tokens._without_tokens(cand), float("nan"))  # not candidates any more
+            else:
+                scores = self._score_gathered(Qb, D_tokens, cand)
             rc = lib.tms_mask_candidates(ctypes.c_void_p(scores.data_ptr()), Bq, n_cand, n_cand,
                                          ctypes.c_void_p(cand.data_ptr()),
                                          ctypes.c_void_p(bitmaps.data_ptr()), self.n_docs,
@@ -121,8 +125,6 @@ class IVFIndex:
         kk = min(k, n_cand)
         v, col = topk(scores, kk)  # columns ascend with document id: the tie rule carries over
         pad = torch.isnan(v)  # ranks after every candidate: not a candidate of this query
-        if paged:
-            pad |= v == float("-inf")  # removed from the corpus since the index was built
         vals[:, :kk] = v.masked_fill(pad, float("-inf"))
         ids[:, :kk] = cand[col].masked_fill(pad, -1)
         return vals, ids

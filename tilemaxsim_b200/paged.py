@@ -409,6 +409,10 @@ class PagedCorpus:
         self._host_lengths[ids] = 0
         self.n_free += freed
 
+    def _without_tokens(self, doc_ids: torch.Tensor) -> torch.Tensor:
+        """Which of the documents doc_ids (n,), ids of the corpus on its device, are removed or empty: (n,) bool."""
+        return self._lengths[doc_ids] == 0
+
     def _count_offsets(self) -> None:
         self._page_offsets[1:] = torch.cumsum((self._lengths + self.page_size - 1) // self.page_size, 0)
         self._token_offsets[1:] = torch.cumsum(self._lengths, 0)
