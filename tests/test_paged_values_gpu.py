@@ -161,3 +161,53 @@ def test_scores_find_every_element_of_a_query(page, d, bq, nq, dtype, cuda_devic
     bound = (big * 2.0 ** -21 + q.abs() * (nq + 4) * 2.0 ** -23).sum(1)
     off = (got - q.sum(1)).abs()
     assert (off <= bound).all(), (off / bound).max()
+
+
+def _row_beside_a_scale_midpoint(rng, d, rms, above):
+    """An fp32 row whose largest |y| over 448 lies within 2^-44 of the middle between two fp32 numbers, on the
+    side asked for: one small element is chosen to bring the norm there. None where it does not come near.
+    Nearer than 2^-49 is left out: in 64 bits a sum of squares takes at most 13 roundings of 2^-53 one after the
+    other (8 fmas, 5 exchanges), of which the root keeps half, and the root, the mean, the quotient and 1 / 448
+    one or two each: under 11 * 2^-53 = 2^-49.5."""
+    L = np.longdouble
+    x = np.clip(rng.normal(size=d), -3.5, 3.5).astype(np.float32)
+    top = np.float32(4 + rng.random())
+    x[0], x[1] = top, 0
+    rest = (x.astype(L) ** 2).sum()
+    mean = L(d) if rms else L(1)
+    s = L(top) / np.sqrt(rest / mean) / 448
+    low = np.nextafter(np.float32(s), np.float32(0))
+    low = np.nextafter(low, np.float32(0))
+    middle = (L(low) + L(np.nextafter(low, np.float32(1)))) / 2
+    need = (L(top) / (448 * middle)) ** 2 * mean - rest
+    x[1] = np.float32(np.sqrt(need))
+    for _ in range(4):
+        s = L(top) / np.sqrt((x.astype(L) ** 2).sum() / mean) / 448
+        off = (s - middle) / middle
+        if 2.0 ** -49 < abs(off) < 2.0 ** -44 and (off > 0) == above:
+            return x, np.float32(low) if off < 0 else np.nextafter(low, np.float32(1))
+        x[1] = np.nextafter(x[1], np.float32(0 if off < 0 else 1))
+    return None
+
+
+@pytest.mark.parametrize("above", [False, True])
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("d,page", [(16, 16), (64, 32), (128, 32), (256, 128)])
+def test_write_scales_beside_a_midpoint(d, page, rms, above, cuda_device):
+    """The scale is rounded once, from what 64 bits give, also where that is next to the middle of two fp32
+    numbers: rows of one-token documents, checked in 80 bits."""
+    from tilemaxsim_b200 import page_tables, page_write
+    rng = np.random.default_rng(d)
+    rows, want = [], []
+    for _ in range(20000):
+        if (r := _row_beside_a_scale_midpoint(rng, d, rms, above)) is not None:
+            rows.append(r[0])
+            want.append(r[1])
+        if len(rows) == 64:
+            break
+    n = len(rows)
+    assert n == 64
+    t = page_tables(torch.ones(n, dtype=torch.int64, device=cuda_device), page, torch.arange(n, dtype=torch.int32, device=cuda_device), n)
+    codes, scales = _pool(n, page, d)
+    page_write(torch.from_numpy(np.stack(rows)).cuda(), t, codes, scales, norm="rms" if rms else "l2", eps=0.0)
+    np.testing.assert_array_equal(scales.cpu().numpy(), np.array(want))

@@ -411,26 +411,30 @@ struct Eight {
 // The scale is the fp32 rounding, and every code the e4m3 rounding, of what 64 bits give, at little
 // more than fp32's cost. fp32 gives every row's factor to 2^-21. Only rows whose largest magnitude
 // comes within 2^-19 of the page's can set the scale: they (one, as a rule) are summed again in
-// fp64. A code is that of t = h * w * factor / scale: where t * (1 - 2^-20) and t * (1 + 2^-20)
+// fp64, which brings their factors to 2^-41, and have fp64's own root where that leaves the scale
+// open. A code is that of t = h * w * factor / scale: where t * (1 - 2^-20) and t * (1 + 2^-20)
 // round to the same one, fp32 is sure of it; the others (about one of 4,000 groups of eight
 // elements) are done again in fp64, with its root and a division: whole numbers of a rational length
-// have exact ties, which a factor 2^-42 off would break to one side. Where nothing is normalised, added or weighted,
-// ties are common and exact, and one fp32 division with its remainder decides them (5,000 documents:
-// 164 us; fp64's took a quarter more). Pages that hold a magnitude or a sum of squares outside [1e-30,
-// 1e30], zeros apart, go through fp64 altogether; NaN and infinities are found there.
+// have exact ties, which a factor 2^-42 off would break to one side. Where nothing is normalised,
+// added or weighted, ties are common and exact, and one fp32 division with its remainder decides them
+// (5,000 documents: 164 us; fp64's took a quarter more). Pages that hold a magnitude or a sum of
+// squares outside [1e-30, 1e30], zeros apart, go through fp64 altogether; NaN and infinities are found
+// there.
 //
-// 20,000 documents (3.6M tokens, 128 bf16 values, unit length) take 452 us, 3.1 TB/s. Neither memory nor
+// 20,000 documents (3.6M tokens, 128 bf16 values, unit length) take 454 us, 3.1 TB/s. Neither memory nor
 // issue slots (62% busy) are full: with 21 warps an SM, a warp waits for its CTA's barriers, for fixed
 // latencies and for shared memory, in about equal parts. Fewer instructions help all the same: with the
 // width as a constant of the kernel where it is 128 (D) that took a sixth less, and 1,600 pages with a
-// residual 14.9 us against 17; the page size as a constant too would give 2% more. Before, rows held in registers took 770 us (few warps fit), all
-// sums in fp64 600-820, sixteen elements a lane 546, fp64 roots for the rows that set the scale 830.
+// residual 14.9 us against 17; the page size as a constant too would give 2% more. The look whether the
+// scale is open takes 3 us (20 of 1,050 at d = 256). Before, rows held in registers took 770 us (few warps
+// fit), all sums in fp64 600-820, sixteen elements a lane 546, fp64 roots for all rows that can set the
+// scale 830.
 __device__ __forceinline__ double max_keep_nan(double x, double y) { return y <= x || x != x ? x : y; }
 __device__ __forceinline__ bool usual(float v) { return v >= 1e-30f && v <= 1e30f; }
 
 // Threads of a CTA: 32 where a page's input is 4 KB at most, 64 up to 8 KB, else 128: as many CTAs as
 // shared memory has stages for then have warps enough, and few warps a page wait for one another
-// little. 3.64M tokens of bf16: d = 64 288 us with 32 threads, 342 with 64; pages of 16 468 and 572;
+// little. 3.64M tokens of bf16, before the look at open scales: d = 64 288 us with 32 threads, 342 with 64; pages of 16 468 and 572;
 // pages of 32 515 with 32, 452 with 64, 548 with 128; pages of 64 538 with 64, 456 with 128; d = 256
 // 1,232 and 1,030. 1,024 documents with a residual (16 KB a page): 52 us with 64, 45 with 128.
 constexpr int write_threads(int input) { return input <= 4096 ? 32 : input <= 8192 ? 64 : 128; }
@@ -448,6 +452,15 @@ __device__ __forceinline__ float off_midpoint(float h, float scale) {
   const float rest = fmaf(-q, scale, h);  // exact
   if (rest == 0.f) return q;
   return __uint_as_float(__float_as_uint(q) + ((rest > 0.f) == (q > 0.f) ? 1u : 0xffffffffu));
+}
+
+__device__ __forceinline__ double scale_of(double y) { return y * (1.0 / kE4m3Max); }
+// Whether scale_of(y), y off by 2^-41 at most, rounds to fp32 for certain: its 29 bits below fp32's are not
+// within 2^13 of the middle, and fp32 has it as a normal number.
+__device__ __forceinline__ bool sure_scale(double y) {
+  const double s = scale_of(y);
+  const int below = __double2loint(s) & 0x1fffffff;
+  return abs(below - 0x10000000) > 0x2000 && s > 1.2e-38;
 }
 
 struct Entry {    // where a table entry's rows come from
@@ -728,9 +741,13 @@ page_write_kernel(const WriteArgs a, int lanes) {
         const int r = base + __ffs(might) - 1;
         might &= might - 1;
         ExactRow exact;
-        exact_row(rows, e, r, row_factor[r], odd, exact);
+        double y;
+        for (bool full = odd;; full = true) {  // the same for all lanes
+          exact_row(rows, e, r, row_factor[r], full, exact);
+          y = full ? exact.top / exact.norm : exact.top * exact.factor;
+          if (full || sure_scale(y)) break;
+        }
         bad |= exact.bad;
-        const double y = odd ? exact.top / exact.norm : exact.top * exact.factor;
         if (y > best) best = y;
       }
     }
@@ -744,7 +761,7 @@ page_write_kernel(const WriteArgs a, int lanes) {
       if (warp_best[i] > best) best = warp_best[i];
       bad |= warp_bad[i] != 0;
     }
-    const float scale = bad ? __int_as_float(0x7fffffff) : static_cast<float>(best * (1.0 / kE4m3Max));
+    const float scale = bad ? __int_as_float(0x7fffffff) : static_cast<float>(scale_of(best));
     const bool plain = !odd && usual(scale);
     const float inverse = __frcp_rn(scale);
     if (threadIdx.x == 0) a.scales[e.id] = scale;
